@@ -3,16 +3,19 @@
     python php-gpu-tensors_b200/build.py            # library + oracle
     python php-gpu-tensors_b200/build.py --force    # rebuild everything
 
-The library is the CUDA translation units csrc/gemm_sm100.cu (kernels and the
-launcher ABI) and csrc/mgpu.cu (multi-GPU entry points, NCCL loaded at run
-time) plus the C++ host layer host/tensor_matmul.cpp, compiled by
-nvcc for compute_100a/sm_100a only, linked with the static CUDA runtime and an export
-map so that only the C ABI of include/gemm_sm100.h is visible.  nvcc
-cross-compiles without a GPU.  The oracle (test infrastructure) is built by
+The library is the CUDA translation units csrc/*.cu (gemm_sm100.cu: matmul
+kernels and the launcher ABI; mgpu.cu: multi-GPU entry points, NCCL loaded at
+run time; the others: the feed-forward layers) plus the C++ host layer
+host/*.cpp, each compiled to an object under build/ by nvcc for
+compute_100a/sm_100a only (in parallel, and only when a source it may include
+changed), linked with the static CUDA runtime and an export map so that only
+the C ABI of include/*.h is visible.  nvcc cross-compiles without a GPU.  The oracle (test infrastructure) is built by
 oracle/Makefile.
 """
+import concurrent.futures
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -23,8 +26,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libgemm_sm100.so")
 HOST = os.path.join(PKG, "host")
-SOURCES = [os.path.join(CSRC, "gemm_sm100.cu"), os.path.join(CSRC, "mgpu.cu"),
-           os.path.join(HOST, "tensor_matmul.cpp")]
+OBJECTS = os.path.join(PKG, "build")
+SOURCES = sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(HOST, "*.cpp")))
 EXPORTS = os.path.join(CSRC, "exports.map")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -56,15 +59,42 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _included(path, seen=None):
+    """`path` and the quoted includes it reaches in csrc/ and include/."""
+    seen = set() if seen is None else seen
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            names = re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M)
+        for name in names:
+            for folder in (CSRC, INCLUDE):
+                if os.path.exists(os.path.join(folder, name)):
+                    _included(os.path.join(folder, name), seen)
+    return seen
+
+
 def build_library(force=False, verbose=False):
     if not force and not _stale(LIB, _sources()):
         return LIB
+    os.makedirs(OBJECTS, exist_ok=True)
+    this = os.path.abspath(__file__)
+    todo, objects = [], []
+    for src in SOURCES:
+        obj = os.path.join(OBJECTS, os.path.basename(src) + ".o")
+        objects.append(obj)
+        if force or _stale(obj, sorted(_included(src)) + [this]):
+            todo.append([nvcc_path()] + NVCC_FLAGS + ["-I", INCLUDE, "-I", CSRC, "-c", src,
+                                                      "-o", obj])
+    with concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        def compile_one(cmd):
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True)
+        list(pool.map(compile_one, todo))
     tmp = LIB + ".tmp"
-    cmd = [nvcc_path()] + NVCC_FLAGS + [
-        "-shared", "-I", INCLUDE, "-I", CSRC,
-        "-Xlinker", "--version-script=" + EXPORTS,
-        "-o", tmp,
-    ] + SOURCES + ["-ldl"]
+    cmd = [nvcc_path()] + ARCH_FLAGS + [
+        "-shared", "-Xcompiler", "-fPIC", "-Xlinker", "--version-script=" + EXPORTS,
+        "-o", tmp] + objects + ["-ldl"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

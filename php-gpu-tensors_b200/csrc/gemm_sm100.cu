@@ -1513,6 +1513,35 @@ __global__ void wait_selftest_kernel(int *status)
 // Internal (hidden) hook for the other translation units of the library.
 void ptg_set_last_status(int code) { set_status(code); }
 
+// Internal (hidden, declared in internal.h), used by the feed-forward kernels.
+bool ptg_device(PtgDevice *out)
+{
+    DeviceState *ds = device_state();
+    if (!ds || ds->cc_major != 10) {
+        set_status(GEMM_SM100_STATUS_NO_DEVICE);
+        return false;
+    }
+    out->sms = ds->sms;
+    out->status = ds->status;
+    return true;
+}
+
+int ptg_precision() { return t_precision; }
+
+void ptg_record_launch(const char *kernel, bool product, int dtype, int grid, int block,
+                       int cluster)
+{
+    if (product) {
+        t_info.builtin_matmul_calls++;
+        t_info.last_matmul = family_name(dtype_code(static_cast<dtype_t>(dtype)));
+    }
+    t_info.last_blas_status = 0;
+    t_last_kernel = kernel;
+    t_last_grid = grid;
+    t_last_block = block;
+    t_last_cluster = cluster;
+}
+
 // Internal (hidden, declared in internal.h), used by csrc/mgpu.cu.
 cudaError_t ptg_launch_f64_peer(const double *a, size_t a_s0, size_t a_s1, const double *b,
                                 size_t b_s0, size_t b_s1, int M, int nb, int K,

@@ -40,3 +40,54 @@ cudaError_t ptg_launch_f64_peer(const double *a, size_t a_s0, size_t a_s1, const
 int ptg_reduced_matmul(const void *a, int a_dtype, const void *b, int b_dtype, float *c,
                        int *shape_a, size_t *stride_a, int nd_a, int *shape_b, size_t *stride_b,
                        int nd_b, int *shape_c, size_t *stride_c, int nd_c, cudaStream_t stream);
+
+// ------------------------------------------------------------ feed-forward
+// Device facts and launch bookkeeping of csrc/gemm_sm100.cu for the other
+// translation units.  ptg_device returns false (and sets the status) without
+// an sm_100 device.
+struct PtgDevice {
+    int sms;
+    int *status;      // device status word
+};
+bool ptg_device(PtgDevice *out);
+int ptg_precision();  // CUDA_MATMUL_PRECISION_* of this thread
+// Names the thread's last kernel and clears its status; a product also counts
+// as a matmul call of `dtype`'s family.
+void ptg_record_launch(const char *kernel, bool product, int dtype, int grid, int block,
+                       int cluster);
+
+// Sets pt_last_error() of this thread and returns `code`; ptg_ok() clears it.
+int ptg_fail(int code, const char *message);
+int ptg_ok();
+
+namespace ptg {
+
+// The rows of a tensor: its leading axes, merged where their strides compose.
+constexpr int kRowViewAxes = 4;
+struct RowView {
+    int n;                              // merged axes, outermost first (at least 1)
+    int ext[kRowViewAxes];
+    long long stride[kRowViewAxes];     // in elements
+};
+
+} // namespace ptg
+
+// Layer norm launches (csrc/layer_norm.cu); arguments are validated by the
+// caller (host/feed_forward.cpp).  dtype is a dtype_t.  Both return a
+// cudaError_t.
+struct PtgLayerNorm {
+    int dtype;
+    const void *x, *grad, *gamma, *beta;
+    int gamma_f32, beta_f32;
+    ptg::RowView xv, gv;
+    long long x_inner, g_inner, rows;
+    int cols;
+    float eps;
+    void *out;
+    float *mean, *rstd;
+    float *dgamma, *dbeta;              // backwards: either may be null
+    float *partial;                     // backwards: workspace
+};
+cudaError_t ptg_layer_norm(const PtgLayerNorm &a, cudaStream_t stream);
+cudaError_t ptg_layer_norm_backward(const PtgLayerNorm &a, cudaStream_t stream);
+size_t ptg_layer_norm_partial_bytes(long long rows, int cols);

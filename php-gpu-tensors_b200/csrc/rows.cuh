@@ -1,0 +1,106 @@
+// Shared by the feed-forward kernels: how a tensor is walked row by row, and
+// how its elements become floats.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "internal.h"
+
+namespace ptg {
+
+// Element offset of row r of a view whose leading axes merged into v.n axes.
+__device__ __forceinline__ long long row_offset(const RowView &v, long long r)
+{
+    if (v.n == 1)
+        return r * v.stride[0];
+    long long off = 0;
+    for (int d = v.n - 1; d >= 0; d--) {
+        off += (r % v.ext[d]) * v.stride[d];
+        r /= v.ext[d];
+    }
+    return off;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v)
+{
+    if constexpr (sizeof(T) == 4)
+        return v;
+    else if constexpr (std::is_same<T, __half>::value)
+        return __half2float(v);
+    else
+        return __bfloat162float(v);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v)
+{
+    if constexpr (sizeof(T) == 4)
+        return v;
+    else if constexpr (std::is_same<T, __half>::value)
+        return __float2half_rn(v);
+    else
+        return __float2bfloat16_rn(v);
+}
+
+// VB bytes of T as one load or store.
+template <int VB>
+struct RawVec;
+template <>
+struct RawVec<16> {
+    using type = uint4;
+};
+template <>
+struct RawVec<8> {
+    using type = uint2;
+};
+template <>
+struct RawVec<4> {
+    using type = uint32_t;
+};
+template <>
+struct RawVec<2> {
+    using type = uint16_t;
+};
+
+template <typename T, int VB>
+__device__ __forceinline__ void unpack_vec(const typename RawVec<VB>::type &raw,
+                                           float (&v)[VB / sizeof(T)])
+{
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < VB / static_cast<int>(sizeof(T)); i++)
+        v[i] = to_float(e[i]);
+}
+
+template <typename T, int VB>
+__device__ __forceinline__ typename RawVec<VB>::type pack_vec(const float (&v)[VB / sizeof(T)])
+{
+    typename RawVec<VB>::type raw;
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < VB / static_cast<int>(sizeof(T)); i++)
+        e[i] = from_float<T>(v[i]);
+    return raw;
+}
+
+// N parameters (gamma, beta, bias) from element i on, in T or in float32.
+template <typename T, int N>
+__device__ __forceinline__ void load_params(const void *p, int is_f32, long long i, float (&v)[N])
+{
+    if (is_f32) {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            v[k] = __ldg(static_cast<const float *>(p) + i + k);
+    } else {
+        constexpr int VB = N * static_cast<int>(sizeof(T));
+        unpack_vec<T, VB>(
+            __ldg(reinterpret_cast<const typename RawVec<VB>::type *>(static_cast<const T *>(p) + i)),
+            v);
+    }
+}
+
+} // namespace ptg

@@ -145,6 +145,14 @@ pt_tensor transposed_view(const pt_tensor *t)
 
 PT_API const char *pt_last_error(void) { return t_error; }
 
+// Internal (hidden, declared in internal.h), used by host/feed_forward.cpp.
+int ptg_fail(int code, const char *message)
+{
+    std::snprintf(t_error, sizeof(t_error), "%s", message);
+    return code;
+}
+int ptg_ok() { return ok(); }
+
 PT_API int pt_matmul_result_shape(const pt_tensor *a, const pt_tensor *b, int *shape, int *ndims)
 {
     if (!a || !b || !shape || !ndims)

@@ -31,7 +31,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libgemm_sm100.so")
 MAX_DIMS = 10
 DTYPE_CODES = {"float32": 0, "float64": 1, "float16": 11, "bfloat16": 12}
 ELEMENT_BYTES = {"float32": 4, "float64": 8, "float16": 2, "bfloat16": 2}
-PT_OK, PT_INVALID_ARGUMENT, PT_RUNTIME = 0, 1, 2
+PT_OK, PT_INVALID_ARGUMENT, PT_RUNTIME, PT_WORKSPACE = 0, 1, 2, 3
 PT_MATMUL_ALLOW_FLOAT64 = 1
 EPILOGUES = {"none": 0, "tanh": 1, "relu": 2, "sigmoid": 3}
 
@@ -72,6 +72,9 @@ class PtTensor(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int), ("ndims", ctypes.c_int),
                 ("shape", ctypes.c_int * MAX_DIMS), ("strides", ctypes.c_size_t * MAX_DIMS)]
 
+
+_PT_TENSOR = struct.Struct("@Pii%di%dN" % (MAX_DIMS, MAX_DIMS))    # pt_tensor's layout
+_PAD = [(0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1)]
 
 _LIB = None
 
@@ -156,6 +159,10 @@ _SIGNATURES = {
     "pt_tensor_release": (None, [ctypes.POINTER(PtTensor), ctypes.c_void_p]),
     "pt_tensor_matmul_backward": (ctypes.c_int, [ctypes.POINTER(PtTensor)] * 5 +
                                   [ctypes.c_void_p]),
+    "pt_layer_norm": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_float] +
+                      [ctypes.c_void_p] * 4),
+    "pt_layer_norm_backward": (ctypes.c_int, [ctypes.c_void_p] * 11),
+    "pt_layer_norm_backward_workspace": (ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
 }
 
 
@@ -180,17 +187,27 @@ def library():
     return _LIB
 
 
+_TORCH = None
+_TORCH_DTYPES = {}     # name -> torch dtype, filled with _TORCH
+_DTYPE_NAMES = {}
+
+
 def _torch():
-    import torch
-    if not torch.cuda.is_available():
-        raise RuntimeException("CUDA device unavailable: CudaArray needs a B200 (sm_100a)")
-    return torch
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        if not torch.cuda.is_available():
+            raise RuntimeException("CUDA device unavailable: CudaArray needs a B200 (sm_100a)")
+        for name in DTYPE_CODES:
+            _TORCH_DTYPES[name] = getattr(torch, name)
+            _DTYPE_NAMES[getattr(torch, name)] = name
+        _TORCH = torch
+    return _TORCH
 
 
 def _torch_dtype(dtype):
-    torch = _torch()
-    return {"float32": torch.float32, "float64": torch.float64, "float16": torch.float16,
-            "bfloat16": torch.bfloat16}[dtype]
+    _torch()
+    return _TORCH_DTYPES[dtype]
 
 
 def _check_dtype(dtype):
@@ -229,12 +246,29 @@ class CudaArray:
 
     def __init__(self, storage, shape, strides=None, offset=0, dtype="float32"):
         _check_dtype(dtype)
-        self._storage = storage            # 1-D torch tensor of the dtype
+        self._flat = storage               # 1-D torch tensor of the dtype
+        self._tensor = None
         self._shape = [int(d) for d in shape]
         self._strides = [int(s) for s in (strides if strides is not None
                                           else _contiguous_strides(self._shape))]
         self._offset = int(offset)
         self._dtype = dtype
+
+    @property
+    def _storage(self):
+        """The whole storage as a 1-D torch tensor (of a wrapped tensor made
+        when it is first asked for)."""
+        if self._flat is None:
+            t = self._tensor
+            n = t.untyped_storage().nbytes() // t.element_size()
+            self._flat = _torch().as_strided(t, (n,), (1,), 0)
+        return self._flat
+
+    def _address(self):
+        """Device address of the first element."""
+        if self._tensor is not None:
+            return self._tensor.data_ptr()
+        return self._flat.data_ptr() + self._offset * ELEMENT_BYTES[self._dtype]
 
     # ---------------------------------------------------------- constructors
     @classmethod
@@ -258,14 +292,14 @@ class CudaArray:
     @classmethod
     def from_torch(cls, tensor, dtype=None):
         """Wraps a CUDA torch tensor view without copying (storage offset kept)."""
-        torch = _torch()
-        rev = {torch.float32: "float32", torch.float64: "float64", torch.float16: "float16",
-               torch.bfloat16: "bfloat16"}
-        dtype = dtype or rev[tensor.dtype]
-        n = tensor.untyped_storage().nbytes() // tensor.element_size()
-        storage = torch.as_strided(tensor, (n,), (1,), 0)
-        return cls(storage, list(tensor.shape), list(tensor.stride()),
-                   tensor.storage_offset(), dtype)
+        _torch()
+        self = cls.__new__(cls)
+        self._dtype = dtype or _DTYPE_NAMES[tensor.dtype]
+        _check_dtype(self._dtype)
+        self._tensor, self._flat = tensor, None
+        self._shape, self._strides = list(tensor.shape), list(tensor.stride())
+        self._offset = tensor.storage_offset()
+        return self
 
     @classmethod
     def full(cls, shape, value, dtype="float32"):
@@ -306,14 +340,22 @@ class CudaArray:
 
     def _pt(self):
         t = PtTensor()
-        es = ELEMENT_BYTES[self._dtype]
-        t.data = self._storage.data_ptr() + self._offset * es
+        t.data = self._address()
         t.dtype = DTYPE_CODES[self._dtype]
         t.ndims = len(self._shape)
         for i, (d, s) in enumerate(zip(self._shape, self._strides)):
             t.shape[i] = d
             t.strides[i] = s
         return t
+
+    def _packed(self):
+        """The pt_tensor as bytes, which a pointer argument takes as they are."""
+        n = len(self._shape)
+        if n > MAX_DIMS:
+            raise InvalidArgumentException("tensors have at most %d axes" % MAX_DIMS)
+        pad = _PAD[n]
+        return _PT_TENSOR.pack(self._address(), DTYPE_CODES[self._dtype], n, *self._shape, *pad,
+                               *self._strides, *pad)
 
     # ---------------------------------------------------------- matmul
     def matmul(self, other, allow_float64=False):
@@ -371,9 +413,27 @@ class CudaArray:
                                    % info["lastBlasStatus"])
         return result
 
+    # ---------------------------------------------------------- feed-forward
+    def layer_norm(self, gamma=None, beta=None, eps=1e-5, save_stats=False):
+        """Layer norm over the last axis (pt_layer_norm); gamma and beta are
+        [cols] arrays of this dtype or float32.  With save_stats the result is
+        (y, mean, rstd), the float32 statistics layer_norm_backward takes."""
+        _check_feed_forward("layer_norm", self, gamma, beta)
+        y = _result(self._shape, self._dtype)
+        lead = self._shape[:-1]
+        mean = rstd = None
+        if save_stats:
+            mean, rstd = _result(lead, "float32"), _result(lead, "float32")
+        _raise_for(library().pt_layer_norm(
+            _ref(self), _ref(gamma), _ref(beta), eps, _ref(y), _ptr(mean), _ptr(rstd),
+            _raw_stream()))
+        return (y, mean, rstd) if save_stats else y
+
     # ---------------------------------------------------------- export
     def to_torch(self):
         """A torch view of this array (no copy)."""
+        if self._tensor is not None:
+            return self._tensor
         return self._storage.as_strided(self._shape, self._strides, self._offset)
 
     def toArray(self):
@@ -389,6 +449,67 @@ class CudaArray:
         if self._dtype in ("float16", "bfloat16"):
             return t.view(_torch().int16).numpy().view(np.uint16)
         return t.numpy()
+
+
+# ---------------------------------------------------------------- feed-forward
+def _check_feed_forward(what, *arrays):
+    for a in arrays:
+        if a is not None and not isinstance(a, CudaArray):
+            raise InvalidArgumentException("%s operands must be CudaArrays" % what)
+
+
+def _result(shape, dtype):
+    """An uninitialised contiguous array."""
+    torch = _torch()
+    self = CudaArray.__new__(CudaArray)
+    self._dtype, self._flat, self._offset = dtype, None, 0
+    self._tensor = torch.empty(shape, dtype=_TORCH_DTYPES[dtype], device="cuda")
+    self._shape, self._strides = list(shape), _contiguous_strides(shape)
+    return self
+
+
+def _ref(a):
+    """`a` as a pt_tensor argument; None as a null pointer."""
+    return None if a is None else a._packed()
+
+
+def _ptr(a):
+    return None if a is None else a._address()
+
+
+def _raw_stream():
+    torch = _torch()
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _workspace(nbytes):
+    torch = _torch()
+    return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+
+
+def layer_norm_backward(grad, x, gamma, mean, rstd, params=True):
+    """Gradients of CudaArray.layer_norm (pt_layer_norm_backward): (dx, dgamma,
+    dbeta), the last two float32 sums over all rows (None without `params`).
+    mean and rstd are the statistics layer_norm saved."""
+    _check_feed_forward("layer_norm_backward", grad, x, gamma, mean, rstd)
+    lead, cols = x._shape[:-1], x._shape[-1] if x._shape else 0
+    for s in (mean, rstd):
+        if s._dtype != "float32" or s._shape != lead or s._strides != _contiguous_strides(lead):
+            raise InvalidArgumentException(
+                "layer norm statistics must be contiguous float32 arrays, one value a row")
+    dx = _result(x._shape, x._dtype)
+    dgamma = dbeta = work = None
+    lib = library()
+    size = ctypes.c_size_t(0)
+    if params:
+        dgamma, dbeta = _result([cols], "float32"), _result([cols], "float32")
+        size.value = lib.pt_layer_norm_backward_workspace(math.prod(lead), cols)
+        work = _workspace(size.value)
+    _raise_for(lib.pt_layer_norm_backward(
+        _ref(grad), _ref(x), _ref(gamma), _ptr(mean), _ptr(rstd), _ref(dx), _ptr(dgamma),
+        _ptr(dbeta), None if work is None else work.data_ptr(), ctypes.addressof(size),
+        _raw_stream()))
+    return dx, dgamma, dbeta
 
 
 def host_matmul(a, b, c, chunks=8, allow_float64=False, devices=None):
