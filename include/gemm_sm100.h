@@ -211,12 +211,16 @@ int cuda_f64_matmul_nd_launcher(
     int *shape_b, size_t *stride_b, int nd_b,
     int *shape_c, size_t *stride_c, int nd_c, cudaStream_t stream);
 
-/* Activations a fused epilogue can apply (the Fusion plan unary ops). */
+/* Activations a fused epilogue can apply: the Fusion plan's unary ops, and
+ * from GELU on those that only the linear layers of pt_feed_forward.h take. */
 enum {
     CUDA_MATMUL_EPILOGUE_NONE = 0,
     CUDA_MATMUL_EPILOGUE_TANH = 1,
     CUDA_MATMUL_EPILOGUE_RELU = 2,
-    CUDA_MATMUL_EPILOGUE_SIGMOID = 3
+    CUDA_MATMUL_EPILOGUE_SIGMOID = 3,
+    CUDA_MATMUL_EPILOGUE_GELU = 4,      /* z P(z), P the normal distribution function */
+    CUDA_MATMUL_EPILOGUE_GELU_TANH = 5, /* its approximation with tanh */
+    CUDA_MATMUL_EPILOGUE_SILU = 6       /* z sigmoid(z) */
 };
 
 /* Fused native-matmul step: c = act(round(A.B) + bias[N]), the values the
@@ -224,7 +228,8 @@ enum {
  * kernel) produces: the product is rounded to the result dtype, the bias add
  * and activation run in float (double for float64) and round once.  dtype is
  * FLOAT32, FLOAT64, FLOAT16 or BFLOAT16; bias is a contiguous [N] vector of
- * that dtype or NULL; activation is a CUDA_MATMUL_EPILOGUE_* value. */
+ * that dtype or NULL; activation is CUDA_MATMUL_EPILOGUE_NONE, TANH, RELU or
+ * SIGMOID. */
 int cuda_matmul_epilogue_nd_launcher(
     void *a, void *b, void *c, dtype_t dtype,
     int *shape_a, size_t *stride_a, int nd_a,

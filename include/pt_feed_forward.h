@@ -47,6 +47,49 @@ int pt_layer_norm_backward(const pt_tensor *grad, const pt_tensor *x, const pt_t
                            cudaStream_t stream);
 size_t pt_layer_norm_backward_workspace(long long rows, int cols);
 
+/* Linear layer y = activation(x . w + bias) + residual.
+ *
+ * x is [..., K]; its leading axes are the rows.  Without `ends` w is [K, N].
+ * With `ends` the layer is grouped by expert: w is [E, K, N], x is [rows, K]
+ * with the rows sorted by group, and ends, E int32 on the device, holds the
+ * row behind each group's last one (the running sum of the groups' row
+ * counts; an empty group repeats the value before it).  Values that fall or
+ * pass the row count are read as the nearest allowed one; rows behind the
+ * last group belong to none and get zeros.  At most PT_MAX_GROUPS groups.
+ * x, w and residual may have any strides (leading axes as for the layer
+ * norm); operands that the tensor cores' loads cannot describe (no contiguous
+ * axis, rows that do not start at multiples of 16 bytes) are laid out in the
+ * workspace first, and so are the bfloat16 parts of float32 ones.
+ *
+ * bias is contiguous [N] ([E, N]) of x's type or float32; residual has y's
+ * shape and x's type; activation is a CUDA_MATMUL_EPILOGUE_* value.  y and,
+ * unless NULL, pre = x . w + bias, which the backward pass needs for an
+ * activation, are [..., N] of x's type.  Infinite float32 operands can turn
+ * to NaN as in the strict mode of cuda_blas_set_precision.
+ *
+ * *workspace_bytes holds the size of `workspace` (16-byte aligned); where it
+ * is too small the call returns PT_WORKSPACE with the need in its place. */
+#define PT_MAX_GROUPS 2048
+int pt_linear(const pt_tensor *x, const pt_tensor *w, const int *ends, const pt_tensor *bias,
+              int activation, const pt_tensor *residual, const pt_tensor *y,
+              const pt_tensor *pre, void *workspace, size_t *workspace_bytes,
+              cudaStream_t stream);
+
+/* Gradients of pt_linear for the upstream gradient `grad` (y's shape, x's
+ * type): with dz = grad * activation'(pre)
+ *     dx = dz . w^T       [..., K], x's type
+ *     dw = x^T . dz       w's shape (contiguous), x's type or float32
+ *     dbias = column sums of dz, float32 [N] ([E, N])
+ * each unless NULL; the residual's gradient is grad itself.  pre may be NULL
+ * for CUDA_MATMUL_EPILOGUE_NONE.  For 16-bit operands dz is rounded to their
+ * type before the two products (dbias is summed before that); without an
+ * activation grad is used as it is.  Rows of no group take no part, and their
+ * dx is zero; a group without rows has a gradient of zero. */
+int pt_linear_backward(const pt_tensor *grad, const pt_tensor *x, const pt_tensor *w,
+                       const int *ends, const pt_tensor *pre, int activation,
+                       const pt_tensor *dx, const pt_tensor *dw, float *dbias, void *workspace,
+                       size_t *workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,97 @@
+// Activations of the feed-forward layers and their derivatives, in float32.
+//
+//   relu z+            tanh            sigmoid s(z) = 1 / (1 + e^-z)
+//   silu z s(z)        gelu z P(z)     gelu_tanh z s(2 u), u = c (z + 0.044715 z^3)
+//
+// with P the normal distribution function and c = sqrt(2 / pi);
+// (1 + tanh u) / 2 = s(2 u) turns the usual form of gelu_tanh into one
+// exponential and one division.  FAST serves results of 16 bits: the
+// hardware's exponential and division (relative error below 2^-20), two
+// orders under the result's rounding.
+#pragma once
+
+#include "gemm_sm100.h"
+
+namespace ptg {
+
+template <bool FAST>
+__device__ __forceinline__ float exp_of(float x)
+{
+    return FAST ? __expf(x) : expf(x);
+}
+
+template <bool FAST>
+__device__ __forceinline__ float divide(float a, float b)
+{
+    return FAST ? __fdividef(a, b) : a / b;
+}
+
+constexpr float kGeluC = 0.7978845608028654f;     // sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+constexpr float kSqrtHalf = 0.7071067811865476f;
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float activate(float z)
+{
+    if constexpr (ACT == CUDA_MATMUL_EPILOGUE_RELU)
+        return z > 0.0f ? z : 0.0f;
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_TANH)
+        return tanhf(z);
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SIGMOID)
+        return divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-z));
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SILU)
+        return divide<FAST>(z, 1.0f + exp_of<FAST>(-z));
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_GELU)
+        return 0.5f * z * (1.0f + erff(z * kSqrtHalf));
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_GELU_TANH) {
+        const float u = kGeluC * fmaf(kGeluA * z * z, z, z);
+        return divide<FAST>(z, 1.0f + exp_of<FAST>(-2.0f * u));
+    } else
+        return z;
+}
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float activation_slope(float z)
+{
+    if constexpr (ACT == CUDA_MATMUL_EPILOGUE_RELU)
+        return z > 0.0f ? 1.0f : 0.0f;
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_TANH) {
+        const float t = tanhf(z);
+        return fmaf(-t, t, 1.0f);
+    } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SIGMOID) {
+        const float s = divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-z));
+        return s * (1.0f - s);
+    } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SILU) {
+        const float s = divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-z));
+        return s * fmaf(z, 1.0f - s, 1.0f);
+    } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_GELU) {
+        // P(z) + z p(z), p the normal density
+        const float density = exp_of<FAST>(-0.5f * z * z) * (0.5f * kGeluC);
+        return fmaf(z, density, 0.5f * (1.0f + erff(z * kSqrtHalf)));
+    } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_GELU_TANH) {
+        // s + z s (1 - s) 2 u'
+        const float z2 = z * z;
+        const float u = kGeluC * fmaf(kGeluA * z2, z, z);
+        const float s = divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-2.0f * u));
+        const float du = kGeluC * fmaf(3.0f * kGeluA, z2, 1.0f);
+        return fmaf(2.0f * z * s * (1.0f - s), du, s);
+    } else
+        return 1.0f;
+}
+
+// Calls f(integral_constant<int, ACT>) for the run-time activation.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f)
+{
+    switch (act) {
+    case CUDA_MATMUL_EPILOGUE_TANH: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_TANH>()); break;
+    case CUDA_MATMUL_EPILOGUE_RELU: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_RELU>()); break;
+    case CUDA_MATMUL_EPILOGUE_SIGMOID: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_SIGMOID>()); break;
+    case CUDA_MATMUL_EPILOGUE_GELU: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_GELU>()); break;
+    case CUDA_MATMUL_EPILOGUE_GELU_TANH: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_GELU_TANH>()); break;
+    case CUDA_MATMUL_EPILOGUE_SILU: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_SILU>()); break;
+    default: f(std::integral_constant<int, CUDA_MATMUL_EPILOGUE_NONE>()); break;
+    }
+}
+
+} // namespace ptg

@@ -1523,6 +1523,7 @@ bool ptg_device(PtgDevice *out)
     }
     out->sms = ds->sms;
     out->status = ds->status;
+    out->encode = reinterpret_cast<void *>(g_encode);
     return true;
 }
 

@@ -48,6 +48,7 @@ int ptg_reduced_matmul(const void *a, int a_dtype, const void *b, int b_dtype, f
 struct PtgDevice {
     int sms;
     int *status;      // device status word
+    void *encode;     // cuTensorMapEncodeTiled
 };
 bool ptg_device(PtgDevice *out);
 int ptg_precision();  // CUDA_MATMUL_PRECISION_* of this thread
@@ -91,3 +92,40 @@ struct PtgLayerNorm {
 cudaError_t ptg_layer_norm(const PtgLayerNorm &a, cudaStream_t stream);
 cudaError_t ptg_layer_norm_backward(const PtgLayerNorm &a, cudaStream_t stream);
 size_t ptg_layer_norm_partial_bytes(long long rows, int cols);
+
+// Linear layers (csrc/linear.cu): rows in groups, each with its own weight.
+// Arguments are validated by the caller (host/feed_forward.cpp).
+struct PtgLinear {
+    int dtype;                          // dtype_t of x, w, y, grad, dx and pre
+    int groups, rows, inner, cols;      // w is [groups, inner, cols]
+    const int *ends;                    // device, or null for one group of all rows
+    const void *x;
+    ptg::RowView xv;
+    long long x_inner;
+    const void *w;
+    long long w_group, w_inner, w_cols; // element strides
+    int activation;
+    // forwards
+    const void *bias;                   // [groups, cols]
+    int bias_f32;
+    const void *residual;
+    ptg::RowView rv;
+    long long r_inner;
+    void *y;
+    void *pre;                          // written forwards (may be null), read backwards
+    // backwards
+    const void *grad;
+    ptg::RowView gv;
+    long long g_inner;
+    ptg::RowView pv;                    // rows of pre
+    long long p_inner;
+    void *dx, *dw;
+    int dw_dtype;
+    float *dbias;
+    void *workspace;
+    size_t workspace_bytes;
+};
+// Both return a cudaError_t, or cudaErrorMemoryAllocation with *need set and
+// nothing enqueued when the workspace is too small.
+cudaError_t ptg_linear(const PtgLinear &a, size_t *need, cudaStream_t stream);
+cudaError_t ptg_linear_backward(const PtgLinear &a, size_t *need, cudaStream_t stream);

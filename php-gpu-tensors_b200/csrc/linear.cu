@@ -1,0 +1,530 @@
+// Linear layers over groups of rows: which operands TMA can read as they lie,
+// which have to be laid out first, and the launches of ragged_gemm.cuh.
+#include "gemm_sm100.h"
+
+#include "linear.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+using namespace ptg;
+
+namespace {
+
+constexpr size_t kAlign = 256;
+
+long long round8(long long n) { return (n + 7) / 8 * 8; }
+
+int element_bytes(int dtype) { return dtype == DTYPE_FLOAT32 ? 4 : 2; }
+
+// ------------------------------------------------------------ workspace
+// Hands out pieces of the caller's workspace; with no workspace it only
+// counts, so that one plan both sizes and runs a call.
+struct Workspace {
+    uint8_t *base;
+    size_t used;
+    void *take(size_t bytes)
+    {
+        void *p = base ? base + used : nullptr;
+        used += (bytes + kAlign - 1) / kAlign * kAlign;
+        return p;
+    }
+};
+
+// ------------------------------------------------------------ launches
+template <typename Kernel, typename... Args>
+cudaError_t launch(Kernel kernel, dim3 grid, int block, size_t smem, cudaStream_t stream,
+                   Args... args)
+{
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// A rank-5 tiled map; strides in elements of `es` bytes, axes past `rank`
+// have extent 1.
+bool encode(const PtgDevice &dev, CUtensorMap *map, int dtype, const void *base, int rank,
+            const long long *ext, const long long *stride, int box0, int box1)
+{
+    if (!dev.encode)
+        return false;
+    cuuint64_t dims[5], strides[4];
+    cuuint32_t box[5] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(box1), 1, 1, 1};
+    cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+    const cuuint64_t filler = static_cast<cuuint64_t>(round8(ext[0])) * 2;
+    for (int i = 0; i < 5; i++) {
+        dims[i] = i < rank ? static_cast<cuuint64_t>(ext[i]) : 1;
+        if (i > 0)
+            strides[i - 1] = i < rank && dims[i] > 1 ? static_cast<cuuint64_t>(stride[i]) * 2 : filler;
+    }
+    const CUtensorMapDataType type = dtype == DTYPE_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(dev.encode)(
+               map, type, 5, const_cast<void *>(base), dims, strides, box, steps,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+           CUDA_SUCCESS;
+}
+
+// ------------------------------------------------------------ operands
+// A matrix as the product kernels read it: 16-bit, contiguous along one axis,
+// 16-byte aligned, `parts` of them for float32.
+struct Rows {
+    const void *p;
+    long long ld;       // elements between rows
+    long long part;     // elements between parts
+};
+
+struct Weight {
+    const void *p;
+    bool cols_contiguous;
+    long long ld, group, part;
+};
+
+bool aligned(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Whether rows of this view start at multiples of `bytes`.
+bool rows_aligned(const void *p, const RowView &v, int es, int bytes)
+{
+    if (!aligned(p, bytes))
+        return false;
+    for (int d = 0; d < v.n; d++)
+        if (v.ext[d] > 1 && v.stride[d] * es % bytes != 0)
+            return false;
+    return true;
+}
+
+// Launches the layout pass of `rows` rows of `cols` columns.
+cudaError_t lay_out(int dtype, const void *src, const RowView &v, long long inner, long long rows,
+                    int cols, int parts, void *out, const PtgDevice &dev, cudaStream_t stream)
+{
+    LayParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.src = src;
+    p.rows_of = v;
+    p.inner = inner;
+    p.rows = rows;
+    p.cols = cols;
+    p.ld = static_cast<int>(round8(cols));
+    p.out = static_cast<uint16_t *>(out);
+    p.part = rows * p.ld;
+    p.parts = parts;
+    p.vec = inner == 1 && rows_aligned(src, v, element_bytes(dtype), 16);
+    const long long blocks = (rows * (p.ld / 8) + 255) / 256;
+    if (blocks == 0)
+        return cudaSuccess;
+    const dim3 grid(static_cast<unsigned>(std::min<long long>(blocks, dev.sms * 16ll)));
+    if (dtype == DTYPE_FLOAT32)
+        return launch(lay_out_kernel<float>, grid, 256, 0, stream, p);
+    return launch(lay_out_kernel<__half>, grid, 256, 0, stream, p);   // a copy of 16-bit values
+}
+
+// What a call has decided; `run` is false while it is only being sized.
+struct Plan {
+    PtgDevice dev;
+    cudaStream_t stream;
+    Workspace ws;
+    bool run;
+    cudaError_t err;
+    int parts, passes;      // float32: bfloat16 parts and products of them; else 1, 1
+
+    bool ok() const { return err == cudaSuccess; }
+    void then(cudaError_t e)
+    {
+        if (ok())
+            err = e;
+    }
+};
+
+// Rows as they lie if TMA can read them, else laid out in the workspace.
+Rows plan_rows(Plan &pl, int dtype, const void *p, const RowView &v, long long inner,
+               long long rows, int cols)
+{
+    Rows r;
+    r.part = 0;
+    if (dtype != DTYPE_FLOAT32 && v.n == 1 && (inner == 1 || cols == 1) &&
+        (rows == 1 || v.stride[0] > 0) && rows_aligned(p, v, 2, 16)) {
+        r.p = p;
+        r.ld = rows == 1 ? round8(cols) : v.stride[0];
+        return r;
+    }
+    r.ld = round8(cols);
+    r.part = rows * r.ld;
+    void *out = pl.ws.take(static_cast<size_t>(r.part) * pl.parts * 2);
+    r.p = out;
+    if (pl.run && pl.ok())
+        pl.then(lay_out(dtype, p, v, inner, rows, cols, pl.parts, out, pl.dev, pl.stream));
+    return r;
+}
+
+Weight plan_weight(Plan &pl, const PtgLinear &a)
+{
+    Weight w;
+    w.part = 0;
+    const bool cols_first = a.w_cols == 1 || a.cols == 1;
+    const bool inner_first = a.w_inner == 1 || a.inner == 1;
+    if (a.dtype != DTYPE_FLOAT32 && aligned(a.w, 16) &&
+        (a.groups == 1 || (a.w_group % 8 == 0 && a.w_group > 0))) {
+        const bool c = cols_first && (a.inner == 1 || (a.w_inner % 8 == 0 && a.w_inner > 0));
+        const bool k = inner_first && (a.cols == 1 || (a.w_cols % 8 == 0 && a.w_cols > 0));
+        if (c || k) {
+            w.p = a.w;
+            w.cols_contiguous = c;
+            w.ld = c ? (a.inner == 1 ? round8(a.cols) : a.w_inner)
+                     : (a.cols == 1 ? round8(a.inner) : a.w_cols);
+            w.group = a.w_group;
+            return w;
+        }
+    }
+    // laid out along the axis that is contiguous, or else the shorter stride
+    w.cols_contiguous = cols_first || (!inner_first && a.w_cols <= a.w_inner);
+    const int rows = w.cols_contiguous ? a.inner : a.cols;
+    const int cols = w.cols_contiguous ? a.cols : a.inner;
+    RowView v;
+    std::memset(&v, 0, sizeof(v));
+    v.n = 2;
+    v.ext[0] = a.groups;
+    v.stride[0] = a.groups > 1 ? a.w_group : 0;
+    v.ext[1] = rows;
+    v.stride[1] = w.cols_contiguous ? a.w_inner : a.w_cols;
+    w.ld = round8(cols);
+    w.group = rows * w.ld;
+    w.part = w.group * a.groups;
+    void *out = pl.ws.take(static_cast<size_t>(w.part) * pl.parts * 2);
+    w.p = out;
+    if (pl.run && pl.ok())
+        pl.then(lay_out(a.dtype, a.w, v, w.cols_contiguous ? a.w_cols : a.w_inner,
+                        static_cast<long long>(a.groups) * rows, cols, pl.parts, out, pl.dev,
+                        pl.stream));
+    return w;
+}
+
+// ------------------------------------------------------------ products
+constexpr int kMaxDevices = 64;
+
+// CTA pairs of `kernel` that fit the device at one time; raises its
+// shared-memory limit on the first call on a device.  0 on failure.  (The
+// kernel is a template argument: the kernels share one function type.)
+template <auto kernel>
+int pair_count(int sms)
+{
+    static std::mutex mutex;
+    static int counts[kMaxDevices] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices)
+        return 0;
+    std::lock_guard<std::mutex> lock(mutex);
+    if (counts[device])
+        return counts[device];
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRaggedSmem) !=
+        cudaSuccess)
+        return 0;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+    cfg.blockDim = dim3(kRaggedThreads);
+    cfg.dynamicSmemBytes = kRaggedSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+        (void)cudaGetLastError();
+        n = sms / 2;
+    }
+    return counts[device] = n;
+}
+
+template <typename T, bool INNER, bool CHUNKED>
+cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p, long long bound)
+{
+    constexpr auto kernel = ragged_gemm_kernel<T, INNER, CHUNKED>;
+    const int pairs = pair_count<kernel>(pl.dev.sms);
+    if (pairs < 1)
+        return cudaErrorInvalidConfiguration;
+    p.status = pl.dev.status;
+    const long long n = std::max<long long>(1, std::min<long long>(bound, pairs));
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * n));
+    cfg.blockDim = dim3(kRaggedThreads);
+    cfg.dynamicSmemBytes = kRaggedSmem;
+    cfg.stream = pl.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, maps, p);
+}
+
+uint32_t instruction(int dtype, bool a_mn, bool b_mn)
+{
+    const uint32_t fmt = dtype == DTYPE_FLOAT16 ? 0 : 1;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+           (static_cast<uint32_t>(b_mn) << 16) | (16u << 24);      // M = 256
+}
+
+// Rows x weight: `features` columns of the result, `inner` summed over.
+// transposed: the weight's inner axis gives the features (dx).
+cudaError_t product(const Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w,
+                    bool transposed, RaggedParams &p)
+{
+    const int features = transposed ? a.inner : a.cols, inner = transposed ? a.cols : a.inner;
+    p.ends = a.ends;
+    p.groups = a.groups;
+    p.rows = a.rows;
+    p.features = features;
+    p.inner = inner;
+    p.a_mn = transposed ? !w.cols_contiguous : w.cols_contiguous;
+    p.passes = pl.passes;
+    p.idesc = instruction(a.dtype, p.a_mn, false);
+    p.out_row = features;
+    RaggedMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    const long long wext[4] = {p.a_mn ? features : inner, p.a_mn ? inner : features, a.groups,
+                               pl.parts};
+    const long long wstr[4] = {1, w.ld, w.group, w.part};
+    const long long xext[3] = {inner, a.rows, pl.parts};
+    const long long xstr[3] = {1, x.ld, x.part};
+    if (inner > 0 &&
+        (!encode(pl.dev, &maps.a, a.dtype, w.p, 4, wext, wstr, 64, p.a_mn ? 64 : 128) ||
+         !encode(pl.dev, &maps.b, a.dtype, x.p, 3, xext, xstr, 64, 128) ||
+         !encode(pl.dev, &maps.b16, a.dtype, x.p, 3, xext, xstr, 64, 16)))
+        return cudaErrorInvalidValue;
+    const long long bound = static_cast<long long>((features + 255) / 256) *
+                            (a.rows / kRaggedBN + std::min(a.groups, a.rows));
+    switch (a.dtype) {
+    case DTYPE_FLOAT16: return launch_pairs<__half, false, false>(pl, maps, p, bound);
+    case DTYPE_BFLOAT16: return launch_pairs<__nv_bfloat16, false, false>(pl, maps, p, bound);
+    default: return launch_pairs<float, false, true>(pl, maps, p, bound);
+    }
+}
+
+// dw[g] = sum over the rows of group g of x^T dz.
+cudaError_t weight_product(const Plan &pl, const PtgLinear &a, const Rows &x, const Rows &dz,
+                           CUtensorMap *group_maps)
+{
+    RaggedParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.ends = a.ends;
+    p.groups = a.groups;
+    p.rows = a.rows;
+    p.features = a.cols;
+    p.cols = a.inner;
+    p.passes = pl.passes;
+    p.idesc = instruction(a.dtype, true, true);
+    p.out = a.dw;
+    p.out_row = a.cols;
+    p.out_group = static_cast<long long>(a.inner) * a.cols;
+    RaggedMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    auto rows_map = [&](CUtensorMap *map, const Rows &m, int cols) {
+        const long long ext[3] = {cols, a.rows, pl.parts};
+        const long long str[3] = {1, m.ld, m.part};
+        return encode(pl.dev, map, a.dtype, m.p, 3, ext, str, 64, 64);
+    };
+    if (!rows_map(&maps.a, dz, a.cols) || !rows_map(&maps.b, x, a.inner))
+        return cudaErrorInvalidValue;
+    if (a.ends) {
+        p.group_maps = group_maps;
+        const cudaError_t err =
+            launch(group_maps_kernel, dim3(1), 256, static_cast<size_t>(a.groups) * 8, pl.stream,
+                   maps.a, maps.b, a.ends, a.groups, a.rows, group_maps);
+        if (err != cudaSuccess)
+            return err;
+    }
+    const long long bound = static_cast<long long>((a.cols + 255) / 256) *
+                            ((a.inner + kRaggedBN - 1) / kRaggedBN) * a.groups;
+    if (a.dtype == DTYPE_FLOAT32)
+        return launch_pairs<float, true, true>(pl, maps, p, bound);
+    if (a.dtype == DTYPE_FLOAT16) {
+        if (a.dw_dtype == DTYPE_FLOAT32)
+            return launch_pairs<float, true, false>(pl, maps, p, bound);
+        return launch_pairs<__half, true, false>(pl, maps, p, bound);
+    }
+    if (a.dw_dtype == DTYPE_FLOAT32)
+        return launch_pairs<float, true, false>(pl, maps, p, bound);
+    return launch_pairs<__nv_bfloat16, true, false>(pl, maps, p, bound);
+}
+
+bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
+{
+    std::memset(&pl, 0, sizeof(pl));
+    pl.err = cudaSuccess;
+    pl.stream = stream;
+    pl.run = run;
+    if (run && a.workspace)
+        pl.ws.base = reinterpret_cast<uint8_t *>(
+            (reinterpret_cast<uintptr_t>(a.workspace) + kAlign - 1) / kAlign * kAlign);
+    const bool split = a.dtype == DTYPE_FLOAT32;
+    const bool tf32 = ptg_precision() == CUDA_MATMUL_PRECISION_TF32;
+    pl.parts = !split ? 1 : tf32 ? 2 : 3;
+    pl.passes = !split ? 1 : tf32 ? 3 : 6;
+    return !run || ptg_device(&pl.dev);
+}
+
+void forward(Plan &pl, const PtgLinear &a)
+{
+    const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+    const Weight w = plan_weight(pl, a);
+    if (!pl.run || !pl.ok())
+        return;
+    RaggedParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.act = a.activation;
+    p.out = a.y;
+    p.pre = a.pre;
+    p.bias = a.bias;
+    p.bias_f32 = a.bias_f32;
+    p.residual = a.residual;
+    p.residual_rows = a.rv;
+    p.residual_inner = a.r_inner;
+    pl.then(product(pl, a, x, w, false, p));
+}
+
+// Launches slope_kernel and, for dbias, group_sums_kernel.
+void slope(Plan &pl, const PtgLinear &a, void *dz, float *partial)
+{
+    SlopeParams p;
+    std::memset(&p, 0, sizeof(p));
+    const int es = element_bytes(a.dtype);
+    p.grad = a.grad;
+    p.pre = a.pre;
+    p.gv = a.gv;
+    p.pv = a.pv;
+    p.g_inner = a.g_inner;
+    p.p_inner = a.p_inner;
+    p.ends = a.ends;
+    p.groups = a.groups;
+    p.rows = a.rows;
+    p.cols = a.cols;
+    p.act = a.activation;
+    p.g_vec = a.g_inner == 1 && rows_aligned(a.grad, a.gv, es, 16);
+    p.p_vec = a.p_inner == 1 && rows_aligned(a.pre, a.pv, es, 16);
+    p.dz = dz;
+    p.ld = static_cast<int>(round8(a.cols));
+    p.part = static_cast<long long>(a.rows) * p.ld;
+    p.parts = pl.parts;
+    p.partial = partial;
+    p.strips = (a.cols + kSlopeCols - 1) / kSlopeCols;
+    const dim3 grid(static_cast<unsigned>(p.strips) *
+                    (a.rows / kSlopeRows + std::min(a.groups, a.rows)));
+    const size_t table = static_cast<size_t>(a.groups) * 8;
+    switch (a.dtype) {
+    case DTYPE_FLOAT16: pl.then(launch(slope_kernel<__half>, grid, 256, table, pl.stream, p)); break;
+    case DTYPE_BFLOAT16:
+        pl.then(launch(slope_kernel<__nv_bfloat16>, grid, 256, table, pl.stream, p));
+        break;
+    default: pl.then(launch(slope_kernel<float>, grid, 256, table, pl.stream, p)); break;
+    }
+    if (partial && pl.ok())
+        pl.then(launch(group_sums_kernel, dim3((a.cols + 31) / 32, a.groups), 1024, table,
+                       pl.stream, static_cast<const float *>(partial), a.ends, a.groups, a.rows,
+                       a.cols, a.dbias));
+}
+
+void backward(Plan &pl, const PtgLinear &a)
+{
+    const bool active = a.activation != CUDA_MATMUL_EPILOGUE_NONE;
+    const bool products = a.dx || a.dw;
+    const size_t partial_rows = a.rows / kSlopeRows + std::min(a.groups, a.rows);
+    float *partial = a.dbias ? static_cast<float *>(pl.ws.take(partial_rows * a.cols * 4)) : nullptr;
+    Rows dz;
+    std::memset(&dz, 0, sizeof(dz));
+    if (active || (a.dtype == DTYPE_FLOAT32 && products)) {
+        // float32 without an activation goes through the same kernel, which
+        // then lays out grad's parts and sums its columns in one pass
+        void *out = nullptr;
+        if (products) {
+            dz.ld = round8(a.cols);
+            dz.part = a.rows * dz.ld;
+            out = pl.ws.take(static_cast<size_t>(dz.part) * pl.parts * 2);
+            dz.p = out;
+        }
+        if (pl.run && pl.ok() && (products || a.dbias))
+            slope(pl, a, out, pl.run && a.dbias ? partial : nullptr);
+    } else {
+        if (products)
+            dz = plan_rows(pl, a.dtype, a.grad, a.gv, a.g_inner, a.rows, a.cols);
+        if (a.dbias && pl.run && pl.ok())
+            slope(pl, a, nullptr, partial);
+    }
+    if (a.dx) {
+        const Weight w = plan_weight(pl, a);
+        if (pl.run && pl.ok()) {
+            RaggedParams p;
+            std::memset(&p, 0, sizeof(p));
+            p.out = a.dx;
+            pl.then(product(pl, a, dz, w, true, p));
+        }
+    }
+    if (a.dw) {
+        const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+        CUtensorMap *maps = nullptr;
+        if (a.ends)
+            maps = static_cast<CUtensorMap *>(pl.ws.take(sizeof(CUtensorMap) * 2 * a.groups));
+        if (pl.run && pl.ok())
+            pl.then(weight_product(pl, a, x, dz, maps));
+    }
+}
+
+template <typename F>
+cudaError_t sized_then_run(const PtgLinear &a, size_t *need, cudaStream_t stream, F body)
+{
+    Plan pl;
+    begin(pl, a, false, stream);
+    body(pl, a);
+    *need = pl.ws.used ? pl.ws.used + kAlign : 0;     // its start may have to be moved up
+    if (*need > a.workspace_bytes)
+        return cudaErrorMemoryAllocation;
+    if (!begin(pl, a, true, stream))
+        return cudaErrorNoDevice;
+    body(pl, a);
+    return pl.err;
+}
+
+const char *kernel_of(int dtype)
+{
+    return dtype == DTYPE_FLOAT32   ? "ragged-f32-bf16x3-256x256"
+           : dtype == DTYPE_FLOAT16 ? "ragged-f16-256x256"
+                                    : "ragged-bf16-256x256";
+}
+
+} // namespace
+
+cudaError_t ptg_linear(const PtgLinear &a, size_t *need, cudaStream_t stream)
+{
+    const cudaError_t err = sized_then_run(a, need, stream, forward);
+    if (err == cudaSuccess)
+        ptg_record_launch(kernel_of(a.dtype), true, a.dtype, 0, kRaggedThreads, 2);
+    return err;
+}
+
+cudaError_t ptg_linear_backward(const PtgLinear &a, size_t *need, cudaStream_t stream)
+{
+    const cudaError_t err = sized_then_run(a, need, stream, backward);
+    if (err == cudaSuccess)
+        ptg_record_launch(kernel_of(a.dtype), true, a.dtype, 0, kRaggedThreads, 2);
+    return err;
+}

@@ -1,0 +1,210 @@
+// The passes around the products of the linear layers: operands laid out for
+// TMA, and the gradient of the epilogue.
+#pragma once
+
+#include "activation.cuh"
+#include "gemm_tc.cuh"
+#include "ragged_gemm.cuh"
+#include "rows.cuh"
+
+namespace ptg {
+
+// ------------------------------------------------------------ laying out
+// out[part][row][ld] from a strided source of `rows` rows and `cols` columns,
+// 16 bits an element: a copy (16-bit operands whose strides or alignment TMA
+// cannot describe), or the bfloat16 parts hi, mid, lo of float32 operands.
+// Each thread makes eight neighbouring elements (one 16-byte store); ld is a
+// multiple of 8 and columns behind `cols` are zero.  Bound by memory.
+struct LayParams {
+    const void *src;
+    RowView rows_of;
+    long long inner;        // element stride of the columns
+    long long rows;
+    int cols, ld;
+    uint16_t *out;
+    long long part;         // elements between parts
+    int parts;
+    int vec;                // rows can be read eight elements at a time
+};
+
+__device__ __forceinline__ void store_parts(const float (&v)[8], uint16_t *out, long long part,
+                                            int parts)
+{
+    __nv_bfloat16 h[8], m[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        split3_bf16(v[i], h[i], m[i], l[i]);
+    *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(h);
+    *reinterpret_cast<uint4 *>(out + part) = *reinterpret_cast<const uint4 *>(m);
+    if (parts > 2)
+        *reinterpret_cast<uint4 *>(out + 2 * part) = *reinterpret_cast<const uint4 *>(l);
+}
+
+// Eight elements of a row from column c on; zero from `cols` on.
+template <typename T>
+__device__ __forceinline__ void load8(const T *row, long long inner, int c, int cols, int vec,
+                                      T (&v)[8])
+{
+    if (vec && c + 8 <= cols) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(row + c);
+        uint4 *d = reinterpret_cast<uint4 *>(v);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; i++)
+            d[i] = __ldg(q + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = c + i < cols ? row[(c + i) * inner] : from_float<T>(0.0f);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) lay_out_kernel(const LayParams p)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int per_row = p.ld / 8;
+    const long long total = p.rows * per_row;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const long long r = i / per_row;
+        const int c = static_cast<int>(i - r * per_row) * 8;
+        const T *row = static_cast<const T *>(p.src) + row_offset(p.rows_of, r);
+        alignas(16) T v[8];
+        load8(row, p.inner, c, p.cols, p.vec, v);
+        uint16_t *out = p.out + r * p.ld + c;
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(v);
+        else
+            store_parts(v, out, p.part, p.parts);
+    }
+}
+
+// ------------------------------------------------------------ the epilogue's gradient
+// dz = grad act'(z), rounded once to the operands' type (for the two products
+// behind it: a second rounding of the size of their results'), and the bias
+// gradient, the column sums of dz before that rounding, in float32.  A block
+// takes 64 rows of one group and 256 columns, 8 a thread in 8 row lanes, and
+// writes one partial row; group_sums_kernel adds a group's partial rows in
+// order.  Bound by memory: grad and z read, dz written, each once.
+constexpr int kSlopeRows = 64;
+constexpr int kSlopeCols = 256;
+
+struct SlopeParams {
+    const void *grad, *pre;
+    RowView gv, pv;
+    long long g_inner, p_inner;
+    const int *ends;
+    int groups, rows, cols;
+    int act;
+    int g_vec, p_vec;
+    void *dz;               // [rows][ld]; null when grad itself serves
+    int ld;
+    long long part;         // float32: parts as in lay_out_kernel
+    int parts;
+    float *partial;         // [row tiles][cols], or null
+    int strips;             // column strips: block = row tile * strips + strip
+};
+
+template <typename T, int ACT>
+__device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1, int c, int lane_y,
+                                           float (&sum)[8])
+{
+    constexpr bool kFast = sizeof(T) == 2;
+#pragma unroll 2
+    for (int r = r0 + lane_y; r < r1; r += 8) {
+        alignas(16) T g[8], z[8];
+        load8(static_cast<const T *>(p.grad) + row_offset(p.gv, r), p.g_inner, c, p.cols, p.g_vec,
+              g);
+        if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
+            load8(static_cast<const T *>(p.pre) + row_offset(p.pv, r), p.p_inner, c, p.cols,
+                  p.p_vec, z);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] = to_float(g[i]);
+            if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
+                v[i] *= activation_slope<ACT, kFast>(to_float(z[i]));
+            if (c + i >= p.cols)
+                v[i] = 0.0f;
+            sum[i] += v[i];
+        }
+        if (p.dz && c < p.ld) {
+            uint16_t *out = static_cast<uint16_t *>(p.dz) + static_cast<long long>(r) * p.ld + c;
+            if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint4 *>(out) = pack_vec<T, 16>(v);
+            else
+                store_parts(v, out, p.part, p.parts);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
+{
+    __shared__ float acc[8][kSlopeCols + 8];
+    extern __shared__ int table[];
+    __shared__ int total_end;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    fill_groups(p.ends, p.groups, p.rows, kSlopeRows, table, table + p.groups, &total_end);
+    const GroupTable groups = {table, table + p.groups, p.groups, total_end};
+    const int tile = blockIdx.x / p.strips, strip = blockIdx.x - tile * p.strips;
+    if (tile >= groups.tiles[p.groups - 1])
+        return;
+    const int g = find_group(groups, tile);
+    const int r0 = groups.start[g] + (tile - (g > 0 ? groups.tiles[g - 1] : 0)) * kSlopeRows;
+    const int r1 = min(r0 + kSlopeRows, group_end(groups, g));
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int c = strip * kSlopeCols + x * 8;
+    float sum[8] = {};
+    if (c < p.cols)
+        with_activation(p.act, [&](auto act) { slope_rows<T, act()>(p, r0, r1, c, y, sum); });
+    if (!p.partial)
+        return;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        acc[y][x * 8 + i] = sum[i];
+    __syncthreads();
+    const int col = strip * kSlopeCols + threadIdx.x;
+    if (col < p.cols) {
+        float total = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            total += acc[k][threadIdx.x];
+        p.partial[static_cast<long long>(tile) * p.cols + col] = total;
+    }
+}
+
+// out[g][c] = sum of the partial rows of group g; 32 interleaved sums joined
+// by a fixed tree.  blockIdx.y = g.
+__global__ void __launch_bounds__(1024) group_sums_kernel(const float *partial, const int *ends,
+                                                          int groups, int rows, int cols,
+                                                          float *out)
+{
+    __shared__ float acc[32][33];
+    extern __shared__ int table[];
+    __shared__ int total_end;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    fill_groups(ends, groups, rows, kSlopeRows, table, table + groups, &total_end);
+    const int g = blockIdx.y;
+    const int first = g > 0 ? table[groups + g - 1] : 0, behind = table[groups + g];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + tx;
+    float sum = 0.0f;
+    if (c < cols) {
+#pragma unroll 4
+        for (int k = first + ty; k < behind; k += 32)
+            sum += partial[static_cast<long long>(k) * cols + c];
+    }
+    acc[ty][tx] = sum;
+    __syncthreads();
+    float total = acc[tx][ty];
+    for (int o = 16; o > 0; o >>= 1)
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int oc = blockIdx.x * 32 + ty;
+    if (tx == 0 && oc < cols)
+        out[static_cast<long long>(g) * cols + oc] = total;
+}
+
+} // namespace ptg

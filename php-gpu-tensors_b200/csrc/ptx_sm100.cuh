@@ -126,6 +126,28 @@ __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap *map)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// Tensor maps written on the device: the extent of a map's second axis, the
+// release behind such writes and the acquire in front of a map's use.
+__device__ __forceinline__ void tensor_map_set_dim1(CUtensorMap *map, uint32_t extent)
+{
+    asm volatile("tensormap.replace.tile.global_dim.global.b1024.b32 [%0], 1, %1;" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(extent)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tensor_map_release()
+{
+    asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
+}
+
+__device__ __forceinline__ void tensor_map_acquire(const CUtensorMap *map)
+{
+    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(
+                     reinterpret_cast<uint64_t>(map))
+                 : "memory");
+}
+
 // Makes generic-proxy writes to shared memory visible to the async proxy
 // (TMA stores, tcgen05.mma operand reads).
 __device__ __forceinline__ void fence_proxy_async_smem()

@@ -34,6 +34,8 @@ ELEMENT_BYTES = {"float32": 4, "float64": 8, "float16": 2, "bfloat16": 2}
 PT_OK, PT_INVALID_ARGUMENT, PT_RUNTIME, PT_WORKSPACE = 0, 1, 2, 3
 PT_MATMUL_ALLOW_FLOAT64 = 1
 EPILOGUES = {"none": 0, "tanh": 1, "relu": 2, "sigmoid": 3}
+# activations of the linear layers
+ACTIVATIONS = dict(EPILOGUES, gelu=4, gelu_tanh=5, silu=6)
 
 
 class InvalidArgumentException(ValueError):
@@ -162,6 +164,9 @@ _SIGNATURES = {
     "pt_layer_norm": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_float] +
                       [ctypes.c_void_p] * 4),
     "pt_layer_norm_backward": (ctypes.c_int, [ctypes.c_void_p] * 11),
+    "pt_linear": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int] + [ctypes.c_void_p] * 6),
+    "pt_linear_backward": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int] +
+                           [ctypes.c_void_p] * 6),
     "pt_layer_norm_backward_workspace": (ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
 }
 
@@ -429,6 +434,21 @@ class CudaArray:
             _raw_stream()))
         return (y, mean, rstd) if save_stats else y
 
+    def linear(self, weight, bias=None, activation="none", residual=None, save_pre=False):
+        """activation(self . weight + bias) + residual in one pass (pt_linear):
+        self [..., K], weight [K, N], bias [N], residual [..., N]; activation
+        one of ACTIVATIONS.  With save_pre the result is (y, pre), pre the
+        pre-activation that linear_backward takes."""
+        return _linear(self, weight, None, bias, activation, residual, save_pre)
+
+    def grouped_linear(self, weight, ends, bias=None, activation="none", residual=None,
+                       save_pre=False):
+        """linear with an own weight [E, K, N] and bias [E, N] for each of E
+        groups of consecutive rows of self [rows, K]; ends, an int32 torch
+        tensor on the device, holds the row behind each group's last one."""
+        return _linear(self, weight, _check_ends(ends, weight), bias, activation, residual,
+                       save_pre)
+
     # ---------------------------------------------------------- export
     def to_torch(self):
         """A torch view of this array (no copy)."""
@@ -510,6 +530,79 @@ def layer_norm_backward(grad, x, gamma, mean, rstd, params=True):
         _ptr(dbeta), None if work is None else work.data_ptr(), ctypes.addressof(size),
         _raw_stream()))
     return dx, dgamma, dbeta
+
+
+def _activation_code(activation):
+    if activation not in ACTIVATIONS:
+        raise InvalidArgumentException("Unknown activation %r" % (activation,))
+    return ACTIVATIONS[activation]
+
+
+def _check_ends(ends, weight):
+    torch = _torch()
+    if (not isinstance(ends, torch.Tensor) or ends.dtype != torch.int32 or not ends.is_cuda
+            or ends.dim() != 1 or not ends.is_contiguous()):
+        raise InvalidArgumentException(
+            "ends must be a contiguous int32 vector on the device, one value a group")
+    if isinstance(weight, CudaArray) and weight._shape[:1] != [ends.numel()]:
+        raise InvalidArgumentException("ends must have one value for each of the weight's groups")
+    return ends.data_ptr()
+
+
+def _with_workspace(call):
+    """Runs call(workspace, size) and, where it asks for a workspace, again
+    with one."""
+    size = ctypes.c_size_t(0)
+    status = call(None, ctypes.addressof(size))
+    if status == PT_WORKSPACE:
+        work = _workspace(size.value)
+        status = call(work.data_ptr(), ctypes.addressof(size))
+    _raise_for(status)
+
+
+def _linear(x, weight, ends, bias, activation, residual, save_pre):
+    _check_feed_forward("linear", x, weight, bias, residual)
+    if not x._shape or not weight._shape:
+        raise InvalidArgumentException("linear layers require rows and a weight")
+    code = _activation_code(activation)
+    shape = x._shape[:-1] + weight._shape[-1:]
+    y = _result(shape, x._dtype)
+    pre = _result(shape, x._dtype) if save_pre else None
+    args = (_ref(x), _ref(weight), ends, _ref(bias), code, _ref(residual), _ref(y), _ref(pre))
+    stream, lib = _raw_stream(), library()
+    _with_workspace(lambda work, size: lib.pt_linear(*args, work, size, stream))
+    return (y, pre) if save_pre else y
+
+
+def _linear_backward(grad, x, weight, ends, pre, activation, bias, inputs, weights,
+                     weight_grad_dtype):
+    _check_feed_forward("linear_backward", grad, x, weight, pre)
+    code = _activation_code(activation)
+    dx = _result(x._shape, x._dtype) if inputs else None
+    dw = _result(weight._shape, weight_grad_dtype or x._dtype) if weights else None
+    dbias = _result(weight._shape[:-2] + weight._shape[-1:], "float32") if bias else None
+    args = (_ref(grad), _ref(x), _ref(weight), ends, _ref(pre), code, _ref(dx), _ref(dw),
+            _ptr(dbias))
+    stream, lib = _raw_stream(), library()
+    _with_workspace(lambda work, size: lib.pt_linear_backward(*args, work, size, stream))
+    return dx, dw, dbias
+
+
+def linear_backward(grad, x, weight, pre=None, activation="none", bias=True, inputs=True,
+                    weights=True, weight_grad_dtype=None):
+    """Gradients of CudaArray.linear (pt_linear_backward): (dx, dw, dbias), each
+    None where it is not wanted (inputs, weights, bias).  pre is what
+    linear(save_pre=True) kept; dw has weight's type or float32, dbias is
+    float32; the residual's gradient is grad itself."""
+    return _linear_backward(grad, x, weight, None, pre, activation, bias, inputs, weights,
+                            weight_grad_dtype)
+
+
+def grouped_linear_backward(grad, x, weight, ends, pre=None, activation="none", bias=True,
+                            inputs=True, weights=True, weight_grad_dtype=None):
+    """Gradients of CudaArray.grouped_linear, as linear_backward."""
+    return _linear_backward(grad, x, weight, _check_ends(ends, weight), pre, activation, bias,
+                            inputs, weights, weight_grad_dtype)
 
 
 def host_matmul(a, b, c, chunks=8, allow_float64=False, devices=None):

@@ -1,0 +1,385 @@
+"""Linear layers, plain and grouped by expert (include/pt_feed_forward.h),
+against float64, element by element.
+
+Tolerances, with u the unit roundoff of the operands' type and A = |x| . |w|
+the magnitudes a dot product of length K adds: products of 16-bit values are
+exact in float32 and the tensor core truncates its sum, so a product is within
+(K + 8) 2^-23 A; float32 operands lose less than 2^-22 A in their parts as
+well.  Activations have slopes below 1.2 and are computed to 2^-16 of their
+argument (16-bit results) or 2^-20.  A result is rounded once, and backwards
+the 16-bit dz once before it, which moves a product by at most u |dz| . |w|.
+"""
+import ctypes
+import math
+
+import pytest
+
+import phptensors as P
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+
+DT = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
+UNIT = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+TINY = {"float32": 0.0, "float16": 2.0 ** -25, "bfloat16": 0.0}
+ALL = ["bfloat16", "float16", "float32"]
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    if torch.cuda.is_available():
+        assert P.device_status() == 0
+
+
+def arr(t):
+    return None if t is None else P.CudaArray.from_torch(t)
+
+
+def act64(z, name):
+    F = torch.nn.functional
+    return {"none": lambda: z, "relu": lambda: F.relu(z), "tanh": lambda: torch.tanh(z),
+            "sigmoid": lambda: torch.sigmoid(z), "silu": lambda: F.silu(z),
+            "gelu": lambda: F.gelu(z), "gelu_tanh": lambda: F.gelu(z, approximate="tanh")}[name]()
+
+
+def slope64(z, name):
+    z = z.clone().requires_grad_()
+    return torch.autograd.grad(act64(z, name).sum(), z)[0]
+
+
+def product_slack(k, dtype):
+    return (k + 8) * 2.0 ** -23 + (2.0 ** -22 if dtype == "float32" else 0.0)
+
+
+def act_slack(z, dtype):
+    return (2.0 ** -16 if UNIT[dtype] > 2.0 ** -20 else 2.0 ** -20) * z.abs()
+
+
+def strided(t, layout):
+    """The values of t in another layout."""
+    if layout == "column":
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    if layout == "padded":          # rows at an odd pitch, off by one element
+        shape = list(t.shape)
+        shape[-1] += 3
+        base = torch.full(shape, float("nan"), dtype=t.dtype, device=t.device)
+        base[..., 1:1 + t.shape[-1]] = t
+        return base[..., 1:1 + t.shape[-1]]
+    if layout == "gaps":            # every second element
+        base = torch.zeros(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype, device=t.device)
+        base[..., ::2] = t
+        return base[..., ::2]
+    return t
+
+
+def spans_of(ends, rows):
+    spans, at = [], 0
+    for e in ends:
+        e = min(max(e, at), rows)
+        spans.append((at, e))
+        at = e
+    return spans
+
+
+def case(rows, inner, cols, dtype, seed, groups=None, layout="plain"):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rnd(*shape, scale=1.0):
+        return strided((torch.randn(*shape, generator=g, device="cuda") * scale).to(DT[dtype]),
+                       layout)
+    lead = [] if groups is None else [groups]
+    return {"x": rnd(rows, inner), "w": rnd(*lead, inner, cols, scale=inner ** -0.5),
+            "bias": (torch.randn(*lead, cols, generator=g, device="cuda") * 0.5).to(DT[dtype]),
+            "res": rnd(rows, cols), "grad": rnd(rows, cols), "pre": rnd(rows, cols)}
+
+
+def check_forward(c, y, pre, dtype, act, spans, bias=True, res=True):
+    x, w = c["x"].double(), c["w"].double().reshape(len(spans), *c["w"].shape[-2:])
+    y, pre = y.double(), None if pre is None else pre.double()
+    for e, (a, b) in enumerate(spans):
+        z = x[a:b] @ w[e]
+        mag = x[a:b].abs() @ w[e].abs()
+        if bias:
+            be = c["bias"].double().reshape(len(spans), -1)[e]
+            z, mag = z + be, mag + be.abs()
+        slack = product_slack(x.shape[1], dtype) * mag + TINY[dtype]
+        want = act64(z, act)
+        if pre is not None:
+            assert torch.all((pre[a:b] - z).abs() <= slack + UNIT[dtype] * z.abs()), (act, e)
+        if res:
+            want = want + c["res"][a:b].double()
+        tol = 1.2 * slack + act_slack(z, dtype) + UNIT[dtype] * want.abs()
+        tol = tol * (1 + 2 * UNIT[dtype]) + (2.0 ** -23 * c["res"][a:b].double().abs() if res else 0)
+        assert torch.all((y[a:b] - want).abs() <= tol), (act, e)
+    rest = spans[-1][1]
+    assert not y[rest:].any() and (pre is None or not pre[rest:].any())
+
+
+def check_backward(c, out, dtype, act, spans, dw_dtype=None):
+    dx, dw, db = [t.to_torch().double() for t in out]
+    x, w = c["x"].double(), c["w"].double().reshape(len(spans), *c["w"].shape[-2:])
+    u = UNIT[dtype]
+    dw, db = dw.reshape(w.shape), db.reshape(len(spans), -1)
+    for e, (a, b) in enumerate(spans):
+        z, grad = c["pre"][a:b].double(), c["grad"][a:b].double()
+        slope = slope64(z, act) if act != "none" else torch.ones_like(z)
+        dz = grad * slope
+        off = grad.abs() * 4 * act_slack(z.abs() + 1, dtype) if act != "none" else 0 * grad
+        mag = dz.abs() + off
+        # dz: its activation's error, and its rounding when it is one
+        dz_off = off + (u * mag if act != "none" and dtype != "float32" else 0) + TINY[dtype]
+        k = w.shape[2]
+        tol = dz_off @ w[e].abs().T + product_slack(k, dtype) * (mag @ w[e].abs().T)
+        want = dz @ w[e].T
+        assert torch.all((dx[a:b] - want).abs() <= tol * (1 + u) + u * want.abs() + TINY[dtype]), e
+        tol = x[a:b].abs().T @ dz_off + product_slack(b - a, dtype) * (x[a:b].abs().T @ mag)
+        want = x[a:b].T @ dz
+        ud = UNIT[dw_dtype or dtype]
+        assert torch.all((dw[e] - want).abs()
+                         <= tol * (1 + ud) + ud * want.abs() + TINY[dtype]), e
+        tol = off.sum(0) + (b - a + 64) * 2.0 ** -24 * mag.sum(0)
+        assert torch.all((db[e] - dz.sum(0)).abs() <= tol), e
+    assert not dx[spans[-1][1]:].any()
+
+
+SIZES = [(1, 64, 64), (2, 8, 8), (3, 7, 5), (8, 128, 264), (31, 65, 1), (33, 1, 70), (129, 72, 520),
+         (256, 256, 256), (257, 200, 96), (300, 1000, 136), (700, 264, 312)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("rows,inner,cols", SIZES)
+def test_linear(dtype, rows, inner, cols):
+    c = case(rows, inner, cols, dtype, rows + inner)
+    for act, bias, res in (("gelu", True, True), ("none", False, False), ("silu", True, False)):
+        y, pre = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]) if bias else None, act,
+                                    arr(c["res"]) if res else None, save_pre=True)
+        check_forward(c, y.to_torch(), pre.to_torch(), dtype, act, [(0, rows)], bias, res)
+    for act in ("gelu", "none"):
+        out = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), act)
+        check_backward(c, out, dtype, act, [(0, rows)])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("act", sorted(P.ACTIVATIONS))
+def test_activations(dtype, act):
+    c = case(70, 96, 200, dtype, 5)
+    c["bias"] = (c["bias"] * 8).contiguous()             # far into both tails
+    c["pre"] = c["pre"] * 4
+    y = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]), act, arr(c["res"]))
+    check_forward(c, y.to_torch(), None, dtype, act, [(0, 70)])
+    out = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), act)
+    check_backward(c, out, dtype, act, [(0, 70)])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ["column", "padded", "gaps"])
+def test_layouts(dtype, layout):
+    c = case(150, 88, 264, dtype, 9, layout=layout)
+    y, pre = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"].float()), "silu", arr(c["res"]),
+                                save_pre=True)
+    check_forward(c, y.to_torch(), pre.to_torch(), dtype, "silu", [(0, 150)])
+    out = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), "silu")
+    check_backward(c, out, dtype, "silu", [(0, 150)])
+    # a residual row that serves every row
+    c["res"] = c["res"][:1].expand(150, 264)
+    y = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]), "silu", arr(c["res"]))
+    check_forward(c, y.to_torch(), None, dtype, "silu", [(0, 150)])
+
+
+ENDS = [[0, 0, 5, 5, 40], [64, 128, 192, 256], [1, 2, 3, 400], [300], [0, 0, 0],
+        [255, 256, 513, 514, 600], [10, 4, 90, 70, 5000]]      # the last one: not in order
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("ends", ENDS)
+@pytest.mark.parametrize("layout", ["plain", "column", "padded"])
+def test_grouped(dtype, ends, layout):
+    rows, inner, cols = max(e for e in ends if e < 5000) + 7, 136, 264
+    c = case(rows, inner, cols, dtype, 21, groups=len(ends), layout=layout)
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    spans = spans_of(ends, rows)
+    # rows of no group hold NaN: nothing of them may reach any result
+    for k in ("x", "grad", "pre", "res"):
+        c[k][spans[-1][1]:] = float("nan")
+    y, pre = arr(c["x"]).grouped_linear(arr(c["w"]), at, arr(c["bias"]), "gelu_tanh",
+                                        arr(c["res"]), save_pre=True)
+    check_forward(c, y.to_torch(), pre.to_torch(), dtype, "gelu_tanh", spans)
+    for act in ("gelu_tanh", "none"):
+        out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at,
+                                        arr(c["pre"]), act)
+        check_backward(c, out, dtype, act, spans)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+def test_nonfinite_rows_stay_in_their_group(dtype):
+    ends = [70, 75, 140]
+    c = case(140, 72, 80, dtype, 4, groups=3)
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    spans = spans_of(ends, 140)
+    for k in ("x", "grad", "res"):
+        c[k][70:75] = float("nan")
+        c[k][72] = float("inf")
+    y = arr(c["x"]).grouped_linear(arr(c["w"]), at, None, "none", arr(c["res"])).to_torch()
+    dx, dw, db = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at)
+    for t, rows in ((y, True), (dx.to_torch(), True), (dw.to_torch(), False),
+                    (db.to_torch(), False)):
+        bad = t[70:75] if rows else t[1]
+        good = torch.cat([t[:70], t[75:]]) if rows else t[[0, 2]]
+        assert not torch.isfinite(bad).any() and torch.isfinite(good).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_weight_gradient_in_float32(dtype):
+    ends = [33, 33, 200]
+    c = case(200, 96, 168, dtype, 8, groups=3)
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at,
+                                    weight_grad_dtype="float32")
+    assert out[1].dtype() == "float32"
+    check_backward(c, out, dtype, "none", spans_of(ends, 200), dw_dtype="float32")
+
+
+@gpu
+def test_float32_modes():
+    """Strict float32 is near float64 as a whole as well; the tf32 mode keeps
+    16 bits of each operand (parts of 8 and 8: 2^-15 of the magnitudes)."""
+    c = case(400, 2048, 264, "float32", 6)
+    y = arr(c["x"]).linear(arr(c["w"])).to_torch().double()
+    want = c["x"].double() @ c["w"].double()
+    assert (y - want).norm() <= 1e-6 * want.norm()
+    P.cuda_set_matmul_precision("tf32")
+    try:
+        t = arr(c["x"]).linear(arr(c["w"])).to_torch().double()
+    finally:
+        P.cuda_set_matmul_precision("fp32-strict")
+    mag = c["x"].double().abs() @ c["w"].double().abs()
+    assert torch.all((t - want).abs() <= (2.0 ** -15 + 2056 * 2.0 ** -23) * mag)
+
+
+@gpu
+def test_gradient_against_differences():
+    c = case(9, 12, 10, "float32", 2, groups=3)
+    ends = torch.tensor([4, 4, 9], dtype=torch.int32, device="cuda")
+    spans = [(0, 4), (4, 4), (4, 9)]
+    y, pre = arr(c["x"]).grouped_linear(arr(c["w"]), ends, arr(c["bias"]), "gelu", save_pre=True)
+    out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), ends, pre, "gelu")
+    at = [c["x"].double(), c["w"].double(), c["bias"].double()]
+
+    def loss():
+        z = torch.cat([at[0][a:b] @ at[1][e] + at[2][e] for e, (a, b) in enumerate(spans)])
+        return (act64(z, "gelu") * c["grad"].double()).sum()
+    h = 1e-5
+    for k, got in enumerate(out):
+        flat = at[k].reshape(-1)
+        num = torch.empty_like(flat)
+        for i in range(flat.numel()):
+            keep = flat[i].item()
+            flat[i] = keep + h
+            up = loss()
+            flat[i] = keep - h
+            num[i] = (up - loss()) / (2 * h)
+            flat[i] = keep
+        # differences: h^2 times a third derivative of order 10; float32: 1e-5
+        assert torch.allclose(got.to_torch().double().reshape(-1), num, rtol=1e-4, atol=1e-4)
+
+
+@gpu
+def test_ranks_empty_tensors_and_parts_of_the_gradient():
+    c = case(24, 64, 72, "bfloat16", 12)
+    y = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]), "relu").to_torch()
+    x4 = c["x"].view(2, 3, 4, 64).permute(2, 0, 1, 3)
+    y4 = arr(x4).linear(arr(c["w"]), arr(c["bias"]), "relu")
+    assert y4.getShape() == [4, 2, 3, 72]
+    assert torch.equal(y4.to_torch(), y.view(2, 3, 4, 72).permute(2, 0, 1, 3))
+    full = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), "relu")
+    for k, want in enumerate(("inputs", "weights", "bias")):
+        only = {n: n == want for n in ("inputs", "weights", "bias")}
+        got = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), "relu",
+                                **only)
+        assert [t is not None for t in got] == [i == k for i in range(3)]
+        assert torch.equal(got[k].to_torch(), full[k].to_torch())
+    none = c["x"][:0]
+    assert arr(none).linear(arr(c["w"])).getShape() == [0, 72]
+    dx, dw, db = P.linear_backward(arr(c["grad"][:0]), arr(none), arr(c["w"]), arr(c["pre"][:0]),
+                                   "relu")
+    assert not dw.to_torch().any() and not db.to_torch().any()
+    # an inner size of zero leaves the epilogue alone
+    y = arr(c["x"][:, :0]).linear(arr(c["w"][:0]), arr(c["bias"]), "silu", arr(c["res"]))
+    c0 = dict(c, x=c["x"][:, :0], w=c["w"][:0])
+    check_forward(c0, y.to_torch(), None, "bfloat16", "silu", [(0, 24)])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+def test_same_bits_again_on_another_stream_and_in_a_graph(dtype):
+    c = case(500, 328, 264, dtype, 15, groups=4)
+    ends = torch.tensor([100, 101, 380, 500], dtype=torch.int32, device="cuda")
+
+    def both():
+        y, pre = arr(c["x"]).grouped_linear(arr(c["w"]), ends, arr(c["bias"]), "gelu",
+                                            arr(c["res"]), save_pre=True)
+        out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), ends, pre, "gelu")
+        return [t.to_torch() for t in (y, pre, *out)]
+    first = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = both()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            kept = both()
+        graph.replay()
+    side.synchronize()
+    for a, b, k in zip(first, again, kept):
+        assert torch.equal(a, b) and torch.equal(a, k)
+
+
+def _pt(shape, dtype):
+    t = P.PtTensor()
+    t.data, t.dtype, t.ndims = 4096, P.DTYPE_CODES[dtype], len(shape)
+    for i, (d, s) in enumerate(zip(shape, P._contiguous_strides(shape))):
+        t.shape[i], t.strides[i] = d, s
+    return t
+
+
+def test_refusals():
+    """Arguments are refused before any CUDA call."""
+    lib, ref = P.library(), ctypes.byref
+    x, w, y = _pt([4, 8], "float16"), _pt([8, 16], "float16"), _pt([4, 16], "float16")
+    size = ctypes.c_size_t(0)
+
+    def forward(x=x, w=w, ends=None, bias=None, act=0, res=None, y=y, pre=None, work=None):
+        return lib.pt_linear(ref(x), ref(w), ends, bias and ref(bias), act, res and ref(res),
+                             ref(y), pre and ref(pre), work, ref(size), None)
+    strided_y = _pt([4, 16], "float16")
+    strided_y.strides[0] = 32
+    for bad in (dict(x=_pt([4, 8], "float64")), dict(w=_pt([8, 16], "bfloat16")),
+                dict(x=_pt([4, 9], "float16")), dict(y=_pt([5, 16], "float16")),
+                dict(y=_pt([4, 15], "float16")), dict(y=strided_y), dict(act=7), dict(act=-1),
+                dict(bias=_pt([15], "float16")), dict(bias=_pt([16], "bfloat16")),
+                dict(res=_pt([4, 15], "float16")), dict(res=_pt([4, 16], "float32")),
+                dict(pre=_pt([4, 16], "float32")), dict(ends=4096),
+                dict(w=_pt([2, 8, 16], "float16")), dict(work=4097),
+                dict(w=_pt([2049, 8, 16], "float16"), ends=4096),
+                dict(w=_pt([0, 8, 16], "float16"), ends=4096),
+                dict(x=_pt([8], "float16"), y=_pt([16], "float16"))):
+        assert forward(**bad) == P.PT_INVALID_ARGUMENT, bad
+        assert b"linear" in lib.pt_last_error() or b"workspace" in lib.pt_last_error()
+    back = lib.pt_linear_backward
+    assert back(ref(y), ref(x), ref(w), None, None, 4, ref(x), ref(w), None, None, ref(size),
+                None) == P.PT_INVALID_ARGUMENT            # an activation without pre
+    assert back(ref(y), ref(x), ref(w), None, None, 0, ref(x), ref(_pt([8, 16], "bfloat16")), None,
+                None, ref(size), None) == P.PT_INVALID_ARGUMENT
+    # float32 operands need a place for their parts, and say how large
+    x, w, y = _pt([4, 8], "float32"), _pt([8, 16], "float32"), _pt([4, 16], "float32")
+    assert forward(x=x, w=w, y=y) == P.PT_WORKSPACE
+    assert size.value >= 3 * 2 * (4 * 8 + 8 * 16)
+    with pytest.raises(P.InvalidArgumentException):
+        P._activation_code("swish")
