@@ -1528,6 +1528,7 @@ bool ptg_device(PtgDevice *out)
 }
 
 int ptg_precision() { return t_precision; }
+int ptg_path() { return t_path; }
 
 void ptg_record_launch(const char *kernel, bool product, int dtype, int grid, int block,
                        int cluster)

@@ -52,6 +52,7 @@ struct PtgDevice {
 };
 bool ptg_device(PtgDevice *out);
 int ptg_precision();  // CUDA_MATMUL_PRECISION_* of this thread
+int ptg_path();       // gemm_sm100_set_path of this thread
 // Names the thread's last kernel and clears its status; a product also counts
 // as a matmul call of `dtype`'s family.
 void ptg_record_launch(const char *kernel, bool product, int dtype, int grid, int block,

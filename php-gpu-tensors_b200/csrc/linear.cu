@@ -3,6 +3,8 @@
 #include "gemm_sm100.h"
 
 #include "linear.cuh"
+#include "ragged_decode.cuh"
+#include "ragged_simt.cuh"
 
 #include <cudaTypedefs.h>
 
@@ -139,6 +141,7 @@ struct Plan {
     bool run;
     cudaError_t err;
     int parts, passes;      // float32: bfloat16 parts and products of them; else 1, 1
+    const char *kernel;     // of the last product, for gemm_sm100_last_kernel
 
     bool ok() const { return err == cudaSuccess; }
     void then(cudaError_t e)
@@ -169,25 +172,34 @@ Rows plan_rows(Plan &pl, int dtype, const void *p, const RowView &v, long long i
     return r;
 }
 
+// Whether the weight can be read as it lies; describes it in *w if so.
+bool weight_fits(const PtgLinear &a, Weight *w)
+{
+    if (a.dtype == DTYPE_FLOAT32 || !aligned(a.w, 16) ||
+        !(a.groups == 1 || (a.w_group % 8 == 0 && a.w_group > 0)))
+        return false;
+    const bool c = (a.w_cols == 1 || a.cols == 1) &&
+                   (a.inner == 1 || (a.w_inner % 8 == 0 && a.w_inner > 0));
+    const bool k = (a.w_inner == 1 || a.inner == 1) &&
+                   (a.cols == 1 || (a.w_cols % 8 == 0 && a.w_cols > 0));
+    if (w && (c || k)) {
+        w->p = a.w;
+        w->cols_contiguous = c;
+        w->ld = c ? (a.inner == 1 ? round8(a.cols) : a.w_inner)
+                  : (a.cols == 1 ? round8(a.inner) : a.w_cols);
+        w->group = a.w_group;
+    }
+    return c || k;
+}
+
 Weight plan_weight(Plan &pl, const PtgLinear &a)
 {
     Weight w;
     w.part = 0;
+    if (weight_fits(a, &w))
+        return w;
     const bool cols_first = a.w_cols == 1 || a.cols == 1;
     const bool inner_first = a.w_inner == 1 || a.inner == 1;
-    if (a.dtype != DTYPE_FLOAT32 && aligned(a.w, 16) &&
-        (a.groups == 1 || (a.w_group % 8 == 0 && a.w_group > 0))) {
-        const bool c = cols_first && (a.inner == 1 || (a.w_inner % 8 == 0 && a.w_inner > 0));
-        const bool k = inner_first && (a.cols == 1 || (a.w_cols % 8 == 0 && a.w_cols > 0));
-        if (c || k) {
-            w.p = a.w;
-            w.cols_contiguous = c;
-            w.ld = c ? (a.inner == 1 ? round8(a.cols) : a.w_inner)
-                     : (a.cols == 1 ? round8(a.inner) : a.w_cols);
-            w.group = a.w_group;
-            return w;
-        }
-    }
     // laid out along the axis that is contiguous, or else the shorter stride
     w.cols_contiguous = cols_first || (!inner_first && a.w_cols <= a.w_inner);
     const int rows = w.cols_contiguous ? a.inner : a.cols;
@@ -211,13 +223,23 @@ Weight plan_weight(Plan &pl, const PtgLinear &a)
     return w;
 }
 
+// By family (pair, few rows, CUDA cores) and type.
+const char *kernel_name(int family, int dtype)
+{
+    static const char *const names[3][3] = {
+        {"ragged2-bf16x3-256x256", "ragged2-f16-256x256", "ragged2-bf16-256x256"},
+        {"", "ragged-f16-128x64", "ragged-bf16-128x64"},
+        {"ragged-simt-f32", "ragged-simt-f16", "ragged-simt-bf16"}};
+    return names[family][dtype == DTYPE_FLOAT32 ? 0 : dtype == DTYPE_FLOAT16 ? 1 : 2];
+}
+
 // ------------------------------------------------------------ products
 constexpr int kMaxDevices = 64;
 
 // CTA pairs of `kernel` that fit the device at one time; raises its
 // shared-memory limit on the first call on a device.  0 on failure.  (The
 // kernel is a template argument: the kernels share one function type.)
-template <auto kernel>
+template <auto kernel, int THREADS>
 int pair_count(int sms)
 {
     static std::mutex mutex;
@@ -239,7 +261,7 @@ int pair_count(int sms)
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
-    cfg.blockDim = dim3(kRaggedThreads);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = kRaggedSmem;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -255,7 +277,8 @@ template <typename T, bool INNER, bool CHUNKED>
 cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p, long long bound)
 {
     constexpr auto kernel = ragged_gemm_kernel<T, INNER, CHUNKED>;
-    const int pairs = pair_count<kernel>(pl.dev.sms);
+    constexpr int kThreads = ragged_threads(CHUNKED);
+    const int pairs = pair_count<kernel, kThreads>(pl.dev.sms);
     if (pairs < 1)
         return cudaErrorInvalidConfiguration;
     p.status = pl.dev.status;
@@ -270,7 +293,7 @@ cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(2 * n));
-    cfg.blockDim = dim3(kRaggedThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kRaggedSmem;
     cfg.stream = pl.stream;
     cfg.attrs = attr;
@@ -278,16 +301,217 @@ cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p
     return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
 
-uint32_t instruction(int dtype, bool a_mn, bool b_mn)
+// Instruction descriptor without its N field.
+uint32_t instruction(int dtype, bool a_mn, bool b_mn, int m)
 {
     const uint32_t fmt = dtype == DTYPE_FLOAT16 ? 0 : 1;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(a_mn) << 15) |
-           (static_cast<uint32_t>(b_mn) << 16) | (16u << 24);      // M = 256
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// The few-row kernel: how many CTAs share the inner axis of a tile.  As many
+// as keep two CTAs on every SM, and at least four k-blocks for each.
+template <typename T>
+cudaError_t launch_decode(const Plan &pl, const RaggedMaps &maps, RaggedParams &p)
+{
+    constexpr auto kernel = ragged_decode_kernel<T>;
+    static std::mutex mutex;
+    static bool ready[kMaxDevices] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices)
+        return cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (!ready[device]) {
+            const cudaError_t err = cudaFuncSetAttribute(
+                kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(kMaxGroups));
+            if (err != cudaSuccess)
+                return err;
+            ready[device] = true;
+        }
+    }
+    p.status = pl.dev.status;
+    const long long tiles = static_cast<long long>((p.features + 127) / 128) *
+                            (p.ends ? p.rows / kDecodeRows + std::min(p.groups, p.rows)
+                                    : (p.rows + kDecodeRows - 1) / kDecodeRows);
+    const int blocks = (p.inner + 63) / 64;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * pl.dev.sms && blocks >= split * 2 * 4)
+        split *= 2;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+    cfg.blockDim = dim3(kDecodeThreads);
+    cfg.dynamicSmemBytes = decode_smem(p.ends ? p.groups : 0);
+    cfg.stream = pl.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, maps, p, split);
+}
+
+// Few rows: at most half a tile's on average, or two tiles' when the pair
+// kernel would not occupy the GPU once.
+bool few_rows(const PtgDevice &dev, long long pair_tiles, int rows, int groups)
+{
+    return rows <= kDecodeRows / 2 * static_cast<long long>(groups) ||
+           (pair_tiles < dev.sms / 2 && rows <= kDecodeRows * 2ll * groups);
+}
+
+// ------------------------------------------------------------ CUDA cores
+constexpr int kSimtFewRows = 16;
+
+template <typename T, bool INNER, int TF, int TR>
+cudaError_t launch_simt_tile(const Plan &pl, RaggedSimtParams &s)
+{
+    constexpr auto kernel = ragged_simt_kernel<T, INNER, TF, TR>;
+    static std::mutex mutex;
+    static bool ready[kMaxDevices] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices)
+        return cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (!ready[device]) {
+            const cudaError_t err =
+                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     ragged_simt_smem<TF, TR>(kMaxGroups));
+            if (err != cudaSuccess)
+                return err;
+            ready[device] = true;
+        }
+    }
+    const RaggedParams &p = s.p;
+    const long long row_tiles =
+        INNER ? static_cast<long long>((p.cols + TR - 1) / TR) * p.groups
+              : (p.ends ? p.rows / TR + std::min(p.groups, p.rows) : (p.rows + TR - 1) / TR);
+    const long long tiles = row_tiles * ((p.features + TF - 1) / TF);
+    const int steps = ((INNER ? p.rows / p.groups : p.inner) + kSimtStep - 1) / kSimtStep;
+    s.split = 1;
+    while (s.split < 8 && tiles * s.split * 2 <= 4 * pl.dev.sms && steps >= s.split * 2 * 2)
+        s.split *= 2;
+    if (tiles * s.split > 2147483647ll)
+        return cudaErrorInvalidValue;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(s.split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * s.split));
+    cfg.blockDim = dim3(kSimtThreads);
+    cfg.dynamicSmemBytes = ragged_simt_smem<TF, TR>(p.ends ? p.groups : 0);
+    cfg.stream = pl.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.split > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, s);
+}
+
+template <typename T, bool INNER>
+cudaError_t launch_simt(const Plan &pl, RaggedSimtParams &s)
+{
+    const int rows = INNER ? s.p.cols : (s.p.rows + s.p.groups - 1) / s.p.groups;
+    return rows <= kSimtFewRows ? launch_simt_tile<T, INNER, 128, 16>(pl, s)
+                                : launch_simt_tile<T, INNER, 64, 64>(pl, s);
+}
+
+// A matrix of rows with one stride each, in the operands' own type.
+struct Plain {
+    const void *p;
+    long long row, inner;
+};
+
+// Rows x weight as product() does it.
+cudaError_t simt_product(Plan &pl, const PtgLinear &a, const Plain &x, bool transposed,
+                         RaggedParams &p)
+{
+    pl.kernel = kernel_name(2, a.dtype);
+    RaggedSimtParams s;
+    std::memset(&s, 0, sizeof(s));
+    p.ends = a.ends;
+    p.groups = a.groups;
+    p.rows = a.rows;
+    p.features = transposed ? a.inner : a.cols;
+    p.inner = transposed ? a.cols : a.inner;
+    p.out_row = p.features;
+    s.p = p;
+    s.a = x.p;
+    s.a_row = x.row;
+    s.a_inner = x.inner;
+    s.b = a.w;
+    s.b_inner = transposed ? a.w_cols : a.w_inner;
+    s.b_col = transposed ? a.w_inner : a.w_cols;
+    s.b_group = a.w_group;
+    switch (a.dtype) {
+    case DTYPE_FLOAT16: return launch_simt<__half, false>(pl, s);
+    case DTYPE_BFLOAT16: return launch_simt<__nv_bfloat16, false>(pl, s);
+    default: return launch_simt<float, false>(pl, s);
+    }
+}
+
+// dw as weight_product() does it; the result has the operands' type.
+cudaError_t simt_weight_product(Plan &pl, const PtgLinear &a, const Plain &x,
+                                const Plain &dz)
+{
+    pl.kernel = kernel_name(2, a.dtype);
+    RaggedSimtParams s;
+    std::memset(&s, 0, sizeof(s));
+    s.p.ends = a.ends;
+    s.p.groups = a.groups;
+    s.p.rows = a.rows;
+    s.p.features = a.cols;
+    s.p.cols = a.inner;
+    s.p.out = a.dw;
+    s.p.out_row = a.cols;
+    s.p.out_group = static_cast<long long>(a.inner) * a.cols;
+    s.a = x.p;
+    s.a_row = x.inner;
+    s.a_inner = x.row;
+    s.b = dz.p;
+    s.b_inner = dz.row;
+    s.b_col = dz.inner;
+    switch (a.dtype) {
+    case DTYPE_FLOAT16: return launch_simt<__half, true>(pl, s);
+    case DTYPE_BFLOAT16: return launch_simt<__nv_bfloat16, true>(pl, s);
+    default: return launch_simt<float, true>(pl, s);
+    }
+}
+
+// A view's own rows, or a contiguous copy where they have no single stride.
+Plain plan_plain(Plan &pl, int dtype, const void *src, const RowView &v, long long inner,
+                 long long rows, int cols)
+{
+    if (v.n == 1)
+        return {src, v.stride[0], inner};
+    void *out = pl.ws.take(static_cast<size_t>(rows) * cols * element_bytes(dtype));
+    if (pl.run && pl.ok()) {
+        const long long blocks = (rows * cols + 255) / 256;
+        const dim3 grid(static_cast<unsigned>(std::min<long long>(blocks, pl.dev.sms * 16ll)));
+        if (dtype == DTYPE_FLOAT32)
+            pl.then(launch(copy_rows_kernel<float>, grid, 256, 0, pl.stream,
+                           static_cast<const float *>(src), v, inner, rows, cols,
+                           static_cast<float *>(out)));
+        else
+            pl.then(launch(copy_rows_kernel<uint16_t>, grid, 256, 0, pl.stream,
+                           static_cast<const uint16_t *>(src), v, inner, rows, cols,
+                           static_cast<uint16_t *>(out)));
+    }
+    return {out, cols, 1};
+}
+
+// ------------------------------------------------------------ tensor cores
 // Rows x weight: `features` columns of the result, `inner` summed over.
 // transposed: the weight's inner axis gives the features (dx).
-cudaError_t product(const Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w,
+cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w,
                     bool transposed, RaggedParams &p)
 {
     const int features = transposed ? a.inner : a.cols, inner = transposed ? a.cols : a.inner;
@@ -298,7 +522,6 @@ cudaError_t product(const Plan &pl, const PtgLinear &a, const Rows &x, const Wei
     p.inner = inner;
     p.a_mn = transposed ? !w.cols_contiguous : w.cols_contiguous;
     p.passes = pl.passes;
-    p.idesc = instruction(a.dtype, p.a_mn, false);
     p.out_row = features;
     RaggedMaps maps;
     std::memset(&maps, 0, sizeof(maps));
@@ -314,6 +537,14 @@ cudaError_t product(const Plan &pl, const PtgLinear &a, const Rows &x, const Wei
         return cudaErrorInvalidValue;
     const long long bound = static_cast<long long>((features + 255) / 256) *
                             (a.rows / kRaggedBN + std::min(a.groups, a.rows));
+    const int path = ptg_path();
+    const bool few = a.dtype != DTYPE_FLOAT32 && path != 3 &&
+                     (path == 1 || few_rows(pl.dev, bound, a.rows, a.groups));
+    p.idesc = instruction(a.dtype, p.a_mn, false, few ? 128 : 256);
+    pl.kernel = kernel_name(few ? 1 : 0, a.dtype);
+    if (few)
+        return a.dtype == DTYPE_FLOAT16 ? launch_decode<__half>(pl, maps, p)
+                                        : launch_decode<__nv_bfloat16>(pl, maps, p);
     switch (a.dtype) {
     case DTYPE_FLOAT16: return launch_pairs<__half, false, false>(pl, maps, p, bound);
     case DTYPE_BFLOAT16: return launch_pairs<__nv_bfloat16, false, false>(pl, maps, p, bound);
@@ -322,9 +553,10 @@ cudaError_t product(const Plan &pl, const PtgLinear &a, const Rows &x, const Wei
 }
 
 // dw[g] = sum over the rows of group g of x^T dz.
-cudaError_t weight_product(const Plan &pl, const PtgLinear &a, const Rows &x, const Rows &dz,
+cudaError_t weight_product(Plan &pl, const PtgLinear &a, const Rows &x, const Rows &dz,
                            CUtensorMap *group_maps)
 {
+    pl.kernel = kernel_name(0, a.dtype);
     RaggedParams p;
     std::memset(&p, 0, sizeof(p));
     p.ends = a.ends;
@@ -333,7 +565,7 @@ cudaError_t weight_product(const Plan &pl, const PtgLinear &a, const Rows &x, co
     p.features = a.cols;
     p.cols = a.inner;
     p.passes = pl.passes;
-    p.idesc = instruction(a.dtype, true, true);
+    p.idesc = instruction(a.dtype, true, true, 256);
     p.out = a.dw;
     p.out_row = a.cols;
     p.out_group = static_cast<long long>(a.inner) * a.cols;
@@ -384,12 +616,34 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
     return !run || ptg_device(&pl.dev);
 }
 
+// Whether a product runs on the CUDA cores: float32 ones below kSimtWork
+// multiply-adds, 16-bit ones below kSimtLayWork whose operands would have to
+// be laid out first.  The thread's kernel path decides first (2: CUDA cores,
+// 1 and 3: the tensor-core kernels).
+constexpr double kSimtWork = 1.0e9;
+constexpr double kSimtLayWork = 5.0e7;
+
+bool on_cuda_cores(const PtgLinear &a, bool lay)
+{
+    const int path = ptg_path();
+    if (path == 1 || path == 3)
+        return false;
+    const double work = static_cast<double>(a.rows) * a.inner * a.cols;
+    if (path == 2)
+        return true;
+    return a.dtype == DTYPE_FLOAT32 ? work <= kSimtWork : lay && work <= kSimtLayWork;
+}
+
+// Whether the tensor-core kernels would need this call's operands laid out.
+bool needs_layout(const PtgLinear &a, const void *rows, const RowView &v, long long inner, int cols)
+{
+    const bool rows_fit = v.n == 1 && (inner == 1 || cols == 1) &&
+                          (a.rows == 1 || v.stride[0] > 0) && rows_aligned(rows, v, 2, 16);
+    return !rows_fit || !weight_fits(a, nullptr);
+}
+
 void forward(Plan &pl, const PtgLinear &a)
 {
-    const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
-    const Weight w = plan_weight(pl, a);
-    if (!pl.run || !pl.ok())
-        return;
     RaggedParams p;
     std::memset(&p, 0, sizeof(p));
     p.act = a.activation;
@@ -397,14 +651,28 @@ void forward(Plan &pl, const PtgLinear &a)
     p.pre = a.pre;
     p.bias = a.bias;
     p.bias_f32 = a.bias_f32;
-    p.residual = a.residual;
-    p.residual_rows = a.rv;
-    p.residual_inner = a.r_inner;
-    pl.then(product(pl, a, x, w, false, p));
+    if (a.residual) {
+        const Plain r =
+            plan_plain(pl, a.dtype, a.residual, a.rv, a.r_inner, a.rows, a.cols);
+        p.residual = r.p;
+        p.residual_row = r.row;
+        p.residual_inner = r.inner;
+    }
+    if (on_cuda_cores(a, needs_layout(a, a.x, a.xv, a.x_inner, a.inner))) {
+        const Plain x = plan_plain(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+        if (pl.run && pl.ok())
+            pl.then(simt_product(pl, a, x, false, p));
+        return;
+    }
+    const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+    const Weight w = plan_weight(pl, a);
+    if (pl.run && pl.ok())
+        pl.then(product(pl, a, x, w, false, p));
 }
 
-// Launches slope_kernel and, for dbias, group_sums_kernel.
-void slope(Plan &pl, const PtgLinear &a, void *dz, float *partial)
+// Launches slope_kernel and, for dbias, group_sums_kernel; `parts` 0 leaves dz
+// in float32.
+void slope(Plan &pl, const PtgLinear &a, void *dz, int parts, float *partial)
 {
     SlopeParams p;
     std::memset(&p, 0, sizeof(p));
@@ -425,7 +693,7 @@ void slope(Plan &pl, const PtgLinear &a, void *dz, float *partial)
     p.dz = dz;
     p.ld = static_cast<int>(round8(a.cols));
     p.part = static_cast<long long>(a.rows) * p.ld;
-    p.parts = pl.parts;
+    p.parts = parts;
     p.partial = partial;
     p.strips = (a.cols + kSlopeCols - 1) / kSlopeCols;
     const dim3 grid(static_cast<unsigned>(p.strips) *
@@ -448,36 +716,53 @@ void backward(Plan &pl, const PtgLinear &a)
 {
     const bool active = a.activation != CUDA_MATMUL_EPILOGUE_NONE;
     const bool products = a.dx || a.dw;
+    const bool lay = (!active && needs_layout(a, a.grad, a.gv, a.g_inner, a.cols)) ||
+                     needs_layout(a, a.x, a.xv, a.x_inner, a.inner);
+    const bool simt = on_cuda_cores(a, lay) && (!a.dw || a.dw_dtype == a.dtype);
     const size_t partial_rows = a.rows / kSlopeRows + std::min(a.groups, a.rows);
     float *partial = a.dbias ? static_cast<float *>(pl.ws.take(partial_rows * a.cols * 4)) : nullptr;
+
+    // dz in the form that the products read.  float32 on the tensor cores goes
+    // through slope_kernel without an activation too: it then lays out grad's
+    // parts and sums its columns in one pass.
     Rows dz;
+    Plain plain;
     std::memset(&dz, 0, sizeof(dz));
-    if (active || (a.dtype == DTYPE_FLOAT32 && products)) {
-        // float32 without an activation goes through the same kernel, which
-        // then lays out grad's parts and sums its columns in one pass
-        void *out = nullptr;
-        if (products) {
-            dz.ld = round8(a.cols);
-            dz.part = a.rows * dz.ld;
-            out = pl.ws.take(static_cast<size_t>(dz.part) * pl.parts * 2);
-            dz.p = out;
-        }
-        if (pl.run && pl.ok() && (products || a.dbias))
-            slope(pl, a, out, pl.run && a.dbias ? partial : nullptr);
+    std::memset(&plain, 0, sizeof(plain));
+    if (products && (active || (a.dtype == DTYPE_FLOAT32 && !simt))) {
+        dz.ld = round8(a.cols);
+        dz.part = a.rows * dz.ld;
+        const size_t each = a.dtype == DTYPE_FLOAT32 && simt ? 4 : 2 * static_cast<size_t>(pl.parts);
+        void *out = pl.ws.take(static_cast<size_t>(dz.part) * each);
+        dz.p = out;
+        plain = {out, dz.ld, 1};
+        if (pl.run && pl.ok())
+            slope(pl, a, out, simt ? 0 : pl.parts, partial);
     } else {
-        if (products)
+        if (products && simt)
+            plain = plan_plain(pl, a.dtype, a.grad, a.gv, a.g_inner, a.rows, a.cols);
+        else if (products)
             dz = plan_rows(pl, a.dtype, a.grad, a.gv, a.g_inner, a.rows, a.cols);
         if (a.dbias && pl.run && pl.ok())
-            slope(pl, a, nullptr, partial);
+            slope(pl, a, nullptr, 0, partial);
+    }
+    RaggedParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.out = a.dx;
+    if (simt) {
+        if (a.dx && pl.run && pl.ok())
+            pl.then(simt_product(pl, a, plain, true, p));
+        if (a.dw) {
+            const Plain x = plan_plain(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+            if (pl.run && pl.ok())
+                pl.then(simt_weight_product(pl, a, x, plain));
+        }
+        return;
     }
     if (a.dx) {
         const Weight w = plan_weight(pl, a);
-        if (pl.run && pl.ok()) {
-            RaggedParams p;
-            std::memset(&p, 0, sizeof(p));
-            p.out = a.dx;
+        if (pl.run && pl.ok())
             pl.then(product(pl, a, dz, w, true, p));
-        }
     }
     if (a.dw) {
         const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
@@ -501,30 +786,20 @@ cudaError_t sized_then_run(const PtgLinear &a, size_t *need, cudaStream_t stream
     if (!begin(pl, a, true, stream))
         return cudaErrorNoDevice;
     body(pl, a);
+    if (pl.ok())
+        ptg_record_launch(pl.kernel ? pl.kernel : "linear-bias-gradient", pl.kernel != nullptr,
+                          a.dtype, 0, 0, 0);
     return pl.err;
-}
-
-const char *kernel_of(int dtype)
-{
-    return dtype == DTYPE_FLOAT32   ? "ragged-f32-bf16x3-256x256"
-           : dtype == DTYPE_FLOAT16 ? "ragged-f16-256x256"
-                                    : "ragged-bf16-256x256";
 }
 
 } // namespace
 
 cudaError_t ptg_linear(const PtgLinear &a, size_t *need, cudaStream_t stream)
 {
-    const cudaError_t err = sized_then_run(a, need, stream, forward);
-    if (err == cudaSuccess)
-        ptg_record_launch(kernel_of(a.dtype), true, a.dtype, 0, kRaggedThreads, 2);
-    return err;
+    return sized_then_run(a, need, stream, forward);
 }
 
 cudaError_t ptg_linear_backward(const PtgLinear &a, size_t *need, cudaStream_t stream)
 {
-    const cudaError_t err = sized_then_run(a, need, stream, backward);
-    if (err == cudaSuccess)
-        ptg_record_launch(kernel_of(a.dtype), true, a.dtype, 0, kRaggedThreads, 2);
-    return err;
+    return sized_then_run(a, need, stream, backward);
 }

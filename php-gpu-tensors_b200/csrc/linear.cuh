@@ -79,6 +79,20 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const LayParams p)
     }
 }
 
+// A contiguous copy of a view whose rows have no single stride.
+template <typename T>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const T *src, const RowView rows_of,
+                                                        long long inner, long long rows, int cols,
+                                                        T *out)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * cols; i += gridDim.x * 256ll) {
+        const long long r = i / cols;
+        out[i] = src[row_offset(rows_of, r) + (i - r * cols) * inner];
+    }
+}
+
 // ------------------------------------------------------------ the epilogue's gradient
 // dz = grad act'(z), rounded once to the operands' type (for the two products
 // behind it: a second rounding of the size of their results'), and the bias
@@ -105,35 +119,56 @@ struct SlopeParams {
     int strips;             // column strips: block = row tile * strips + strip
 };
 
+// Rows r0 + lane_y + 8 k of one block, four at a time: all their loads are in
+// flight before the first is used.
 template <typename T, int ACT>
 __device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1, int c, int lane_y,
                                            float (&sum)[8])
 {
     constexpr bool kFast = sizeof(T) == 2;
-#pragma unroll 2
-    for (int r = r0 + lane_y; r < r1; r += 8) {
-        alignas(16) T g[8], z[8];
-        load8(static_cast<const T *>(p.grad) + row_offset(p.gv, r), p.g_inner, c, p.cols, p.g_vec,
-              g);
-        if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
-            load8(static_cast<const T *>(p.pre) + row_offset(p.pv, r), p.p_inner, c, p.cols,
-                  p.p_vec, z);
-        float v[8];
+    constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;
+#pragma unroll 1
+    for (int base = r0 + lane_y; base < r1; base += 8 * kBatch) {
+        alignas(16) T g[kBatch][8], z[kBatch][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            v[i] = to_float(g[i]);
+        for (int k = 0; k < kBatch; k++) {
+            const int r = base + 8 * k;
+            if (r >= r1)
+                break;
+            load8(static_cast<const T *>(p.grad) + row_offset(p.gv, r), p.g_inner, c, p.cols,
+                  p.g_vec, g[k]);
             if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
-                v[i] *= activation_slope<ACT, kFast>(to_float(z[i]));
-            if (c + i >= p.cols)
-                v[i] = 0.0f;
-            sum[i] += v[i];
+                load8(static_cast<const T *>(p.pre) + row_offset(p.pv, r), p.p_inner, c, p.cols,
+                      p.p_vec, z[k]);
         }
-        if (p.dz && c < p.ld) {
-            uint16_t *out = static_cast<uint16_t *>(p.dz) + static_cast<long long>(r) * p.ld + c;
-            if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<uint4 *>(out) = pack_vec<T, 16>(v);
-            else
-                store_parts(v, out, p.part, p.parts);
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            const int r = base + 8 * k;
+            if (r >= r1)
+                break;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                v[i] = to_float(g[k][i]);
+                if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
+                    v[i] *= activation_slope<ACT, kFast>(to_float(z[k][i]));
+                if (c + i >= p.cols)
+                    v[i] = 0.0f;
+                sum[i] += v[i];
+            }
+            if (p.dz) {
+                uint16_t *out =
+                    static_cast<uint16_t *>(p.dz) + static_cast<long long>(r) * p.ld + c;
+                if constexpr (sizeof(T) == 2)
+                    *reinterpret_cast<uint4 *>(out) = pack_vec<T, 16>(v);
+                else if (p.parts)
+                    store_parts(v, out, p.part, p.parts);
+                else {
+                    float *o = static_cast<float *>(p.dz) + static_cast<long long>(r) * p.ld + c;
+                    *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4 *>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                }
+            }
         }
     }
 }
@@ -146,14 +181,20 @@ __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
     __shared__ int total_end;
     grid_dependency_wait();
     grid_launch_dependents();
-    fill_groups(p.ends, p.groups, p.rows, kSlopeRows, table, table + p.groups, &total_end);
-    const GroupTable groups = {table, table + p.groups, p.groups, total_end};
     const int tile = blockIdx.x / p.strips, strip = blockIdx.x - tile * p.strips;
-    if (tile >= groups.tiles[p.groups - 1])
+    int r0 = tile * kSlopeRows, end = p.rows;
+    if (p.ends) {
+        fill_groups(p.ends, p.groups, p.rows, kSlopeRows, table, table + p.groups, &total_end);
+        const GroupTable groups = {table, table + p.groups, p.groups, total_end};
+        if (tile >= groups.tiles[p.groups - 1])
+            return;
+        const int g = find_group(groups, tile);
+        r0 = groups.start[g] + (tile - (g > 0 ? groups.tiles[g - 1] : 0)) * kSlopeRows;
+        end = group_end(groups, g);
+    }
+    if (r0 >= end)
         return;
-    const int g = find_group(groups, tile);
-    const int r0 = groups.start[g] + (tile - (g > 0 ? groups.tiles[g - 1] : 0)) * kSlopeRows;
-    const int r1 = min(r0 + kSlopeRows, group_end(groups, g));
+    const int r1 = min(r0 + kSlopeRows, end);
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     const int c = strip * kSlopeCols + x * 8;
     float sum[8] = {};
@@ -186,9 +227,13 @@ __global__ void __launch_bounds__(1024) group_sums_kernel(const float *partial, 
     __shared__ int total_end;
     grid_dependency_wait();
     grid_launch_dependents();
-    fill_groups(ends, groups, rows, kSlopeRows, table, table + groups, &total_end);
     const int g = blockIdx.y;
-    const int first = g > 0 ? table[groups + g - 1] : 0, behind = table[groups + g];
+    int first = 0, behind = (rows + kSlopeRows - 1) / kSlopeRows;
+    if (ends) {
+        fill_groups(ends, groups, rows, kSlopeRows, table, table + groups, &total_end);
+        first = g > 0 ? table[groups + g - 1] : 0;
+        behind = table[groups + g];
+    }
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + tx;
     float sum = 0.0f;

@@ -15,8 +15,8 @@
 // A cluster of two CTAs computes 256 features x up to 256 rows: CTA r loads
 // features [128 r, 128 r + 128) and half of the rows, 64 of K at a time, into
 // a 6-stage ring of 128-byte-swizzled tiles.  Warp 0 issues the TMA loads,
-// warp 1 of CTA 0 the MMAs into one of two 256-column accumulators, warps 2
-// to 9 read the other one, apply bias, activation and residual and store.
+// warp 1 of CTA 0 the MMAs into one of two 256-column accumulators, the other
+// warps read the other one, apply bias, activation and residual and store.
 // Barriers as in gemm_tc2.cuh; every wait is bounded.  No TMA multicast.
 //
 // Ragged INNER axis: a k-block that crosses the end of its group must not
@@ -54,8 +54,7 @@ struct RaggedParams {
     const void *bias;
     int bias_f32;
     const void *residual;
-    RowView residual_rows;
-    long long residual_inner;
+    long long residual_row, residual_inner;   // element strides
     const CUtensorMap *group_maps;      // INNER, several groups: a and b of each group
     int *status;
 };
@@ -69,8 +68,11 @@ struct RaggedMaps {
 constexpr int kMaxGroups = 2048;
 constexpr int kRaggedBN = 256;
 constexpr int kRaggedStages = 6;
-constexpr int kRaggedEpiWarps = 8;
-constexpr int kRaggedThreads = 32 * (2 + kRaggedEpiWarps);
+// Epilogue warps: 16 hide each other's latencies (TMEM, residual, stores);
+// CHUNKED ones keep a tile's sums in registers, which eight warps have room
+// for.
+constexpr int ragged_epi_warps(bool chunked) { return chunked ? 8 : 16; }
+constexpr int ragged_threads(bool chunked) { return 32 * (2 + ragged_epi_warps(chunked)); }
 constexpr int kRaggedTile = 16384;                       // 128 rows x 64 of K, 16 bits
 constexpr int kRaggedRing = kRaggedStages * 2 * kRaggedTile;
 constexpr int kRaggedBars = 2 * kRaggedStages + 4 + 1;
@@ -222,51 +224,77 @@ __device__ __forceinline__ void pass_parts(int passes, int q, int &pa, int &pb)
     pb = (0x046 >> shift) & 3;
 }
 
-// Bias, activation and residual on the values v[j] of rows n0 + j (j < count)
-// at this lane's feature, and their stores: 32 lanes write 32 neighbouring
-// features of one row.
-template <typename T, bool INNER, int N>
-__device__ __forceinline__ void ragged_store(const RaggedParams &p, float (&v)[N], int n0,
-                                             int count, int feature, float bias, T *out, T *pre)
+// The epilogue works on kGroup rows at a time: lane = feature, so a warp
+// reads and writes 32 neighbouring features of each row.
+constexpr int kGroup = 16;
+
+// residual of rows n0 .. n0 + kGroup - 1 (those below count) at this feature.
+template <typename T>
+__device__ __forceinline__ void load_residual(const RaggedParams &p, int n0, int count,
+                                              int feature, T (&r)[kGroup])
+{
+    if (feature >= p.features)
+        return;
+    const T *q = static_cast<const T *>(p.residual) + feature * p.residual_inner +
+                 n0 * p.residual_row;
+    if (count >= kGroup) {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            r[j] = __ldg(q + j * p.residual_row);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            if (j < count)
+                r[j] = __ldg(q + j * p.residual_row);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_group(T *out, long long ld, int count,
+                                            const float (&v)[kGroup])
+{
+    if (count >= kGroup) {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            out[j * ld] = from_float<T>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            if (j < count)
+                out[j * ld] = from_float<T>(v[j]);
+    }
+}
+
+// Bias, activation and residual (r, already loaded) on the values v of rows
+// n0 .. and their stores.
+template <typename T, bool INNER>
+__device__ __forceinline__ void finish_group(const RaggedParams &p, float (&v)[kGroup], int n0,
+                                             int count, int feature, float bias,
+                                             const T (&r)[kGroup], T *out, T *pre)
 {
     constexpr bool kFast = sizeof(T) == 2;
     if (feature >= p.features || count <= 0)
         return;
     const long long ld = p.out_row;
-    out += n0 * ld + feature;
     if constexpr (!INNER) {
 #pragma unroll
-        for (int j = 0; j < N; j++)
+        for (int j = 0; j < kGroup; j++)
             v[j] += bias;
-        if (pre) {
-            pre += n0 * ld + feature;
+        if (pre)
+            store_group(pre + n0 * ld + feature, ld, count, v);
+        if (p.act != CUDA_MATMUL_EPILOGUE_NONE)
+            with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j < count)
-                    pre[j * ld] = from_float<T>(v[j]);
-        }
-        with_activation(p.act, [&](auto act) {
-#pragma unroll
-            for (int j = 0; j < N; j++)
-                v[j] = activate<act(), kFast>(v[j]);
-        });
+                for (int j = 0; j < kGroup; j++)
+                    v[j] = activate<act(), kFast>(v[j]);
+            });
         if (p.residual) {
-            const T *res = static_cast<const T *>(p.residual) + feature * p.residual_inner;
-            T r[N];
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j < count)
-                    r[j] = res[row_offset(p.residual_rows, n0 + j)];
-#pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j < count)
-                    v[j] += to_float(r[j]);
+            for (int j = 0; j < kGroup; j++)
+                v[j] += to_float(r[j]);
         }
     }
-#pragma unroll
-    for (int j = 0; j < N; j++)
-        if (j < count)
-            out[j * ld] = from_float<T>(v[j]);
+    store_group(out + n0 * ld + feature, ld, count, v);
 }
 
 template <typename T>
@@ -319,10 +347,11 @@ __global__ void __launch_bounds__(256)
 }
 
 template <typename T, bool INNER, bool CHUNKED>
-__global__ void __launch_bounds__(kRaggedThreads, 1)
+__global__ void __launch_bounds__(ragged_threads(CHUNKED), 1)
     ragged_gemm_kernel(const __grid_constant__ RaggedMaps maps, const RaggedParams p)
 {
     constexpr int S = kRaggedStages;
+    constexpr int kEpiWarps = ragged_epi_warps(CHUNKED);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -354,7 +383,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], 2 * kRaggedEpiWarps);
+            mbar_init(&tempty[i], 2 * kEpiWarps);
         }
         mbar_init(drain, 1);
         *abort = 0;
@@ -529,8 +558,8 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     } else {
         // ------------------------------------------------------------ epilogue (both CTAs)
         const int quad = warp & 3;                     // TMEM lane quadrant of this warp
-        const int side = (warp - 2) >> 2;              // its 128 of the 256 columns
-        constexpr int kCols = kRaggedBN / 2;
+        const int side = (warp - 2) >> 2;              // its kCols of the 256 columns
+        constexpr int kCols = kRaggedBN / (kEpiWarps / 4);
         long long chunk = 0;
         bool ok = true;
         for (long long t = cluster; ok && t < tiles; t += nclusters) {
@@ -541,8 +570,12 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             T *out = static_cast<T *>(p.out) + (INNER ? r.group * p.out_group : 0);
             T *pre = static_cast<T *>(p.pre);
             float bias = 0.0f;
-            if (!INNER)
+            T res[kGroup];
+            if constexpr (!INNER) {
                 bias = load_bias<T>(p, r.group, feature);
+                if (p.residual && mine > 0)      // in flight while the products run
+                    load_residual(p, n0, r.n_end - n0, feature, res);
+            }
             const int chunks =
                 CHUNKED ? max(1, (r.k_blocks + kChunkBlocks - 1) / kChunkBlocks) : 1;
             float total[CHUNKED ? kCols : 1];
@@ -588,17 +621,29 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     }
                 }
                 if (c == chunks - 1) {
+uint32_t raw[kGroup];
+                    if (mine > 0)
+                        tmem_ld_32x32b_x16(t_acc, raw);
 #pragma unroll 1
-                    for (int h = 0; h < mine; h += 16) {
-                        uint32_t raw[16];
-                        tmem_ld_32x32b_x16(t_acc + h, raw);
+                    for (int h = 0; h < mine; h += kGroup) {
+                        float v[kGroup];
+                        T now[kGroup];
                         tmem_ld_wait_regs(raw);
-                        float v[16];
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
+                        for (int j = 0; j < kGroup; j++) {
                             v[j] = r.k_blocks > 0 ? __uint_as_float(raw[j]) : 0.0f;
-                        ragged_store<T, INNER, 16>(p, v, n0 + h, r.n_end - (n0 + h), feature, bias,
-                                                   out, pre);
+                            now[j] = res[j];
+                        }
+                        if (h + kGroup < mine) {
+                            tmem_ld_32x32b_x16(t_acc + h + kGroup, raw);
+                            if constexpr (!INNER) {
+                                if (p.residual)
+                                    load_residual(p, n0 + h + kGroup, r.n_end - (n0 + h + kGroup),
+                                                  feature, res);
+                            }
+                        }
+                        finish_group<T, INNER>(p, v, n0 + h, r.n_end - (n0 + h), feature, bias, now,
+                                               out, pre);
                         __syncwarp();
                     }
                 }
@@ -609,8 +654,8 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             }
         }
         if (!INNER && groups.end < p.rows)
-            zero_ungrouped<T>(p, groups.end, blockIdx.x * kRaggedEpiWarps + warp - 2,
-                              gridDim.x * kRaggedEpiWarps);
+            zero_ungrouped<T>(p, groups.end, blockIdx.x * kEpiWarps + warp - 2,
+                              gridDim.x * kEpiWarps);
     }
 
     tc_fence_before();

@@ -143,14 +143,27 @@ def check_backward(c, out, dtype, act, spans, dw_dtype=None):
     assert not dx[spans[-1][1]:].any()
 
 
-SIZES = [(1, 64, 64), (2, 8, 8), (3, 7, 5), (8, 128, 264), (31, 65, 1), (33, 1, 70), (129, 72, 520),
+# a case beyond one tile of each kernel in every direction, and odd ones
+SIZES = [(1, 64, 64), (65, 2100, 130), (2, 8, 8), (3, 7, 5), (8, 128, 264), (31, 65, 1), (33, 1, 70), (129, 72, 520),
          (256, 256, 256), (257, 200, 96), (300, 1000, 136), (700, 264, 312)]
 
 
+PATHS = ["auto", "tensor-core", "tensor-core-pair", "simt"]
+
+
+@pytest.fixture
+def path(request):
+    """One of the kernel families: few rows, CTA pairs, CUDA cores."""
+    before = P.set_kernel_path(request.param)
+    yield request.param
+    P.library().gemm_sm100_set_path(before)
+
+
 @gpu
+@pytest.mark.parametrize("path", PATHS, indirect=True)
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("rows,inner,cols", SIZES)
-def test_linear(dtype, rows, inner, cols):
+def test_linear(dtype, rows, inner, cols, path):
     c = case(rows, inner, cols, dtype, rows + inner)
     for act, bias, res in (("gelu", True, True), ("none", False, False), ("silu", True, False)):
         y, pre = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]) if bias else None, act,
@@ -162,9 +175,10 @@ def test_linear(dtype, rows, inner, cols):
 
 
 @gpu
+@pytest.mark.parametrize("path", PATHS[1:], indirect=True)
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("act", sorted(P.ACTIVATIONS))
-def test_activations(dtype, act):
+def test_activations(dtype, act, path):
     c = case(70, 96, 200, dtype, 5)
     c["bias"] = (c["bias"] * 8).contiguous()             # far into both tails
     c["pre"] = c["pre"] * 4
@@ -175,9 +189,10 @@ def test_activations(dtype, act):
 
 
 @gpu
+@pytest.mark.parametrize("path", PATHS[1:], indirect=True)
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("layout", ["column", "padded", "gaps"])
-def test_layouts(dtype, layout):
+def test_layouts(dtype, layout, path):
     c = case(150, 88, 264, dtype, 9, layout=layout)
     y, pre = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"].float()), "silu", arr(c["res"]),
                                 save_pre=True)
@@ -197,8 +212,10 @@ ENDS = [[0, 0, 5, 5, 40], [64, 128, 192, 256], [1, 2, 3, 400], [300], [0, 0, 0],
 @gpu
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("ends", ENDS)
-@pytest.mark.parametrize("layout", ["plain", "column", "padded"])
-def test_grouped(dtype, ends, layout):
+@pytest.mark.parametrize("layout,path", [("plain", p) for p in PATHS] + [
+    ("column", "tensor-core-pair"), ("column", "simt"), ("padded", "tensor-core"),
+    ("padded", "simt")], indirect=["path"])
+def test_grouped(dtype, ends, layout, path):
     rows, inner, cols = max(e for e in ends if e < 5000) + 7, 136, 264
     c = case(rows, inner, cols, dtype, 21, groups=len(ends), layout=layout)
     at = torch.tensor(ends, dtype=torch.int32, device="cuda")
@@ -216,8 +233,9 @@ def test_grouped(dtype, ends, layout):
 
 
 @gpu
+@pytest.mark.parametrize("path", PATHS[1:], indirect=True)
 @pytest.mark.parametrize("dtype", ALL)
-def test_nonfinite_rows_stay_in_their_group(dtype):
+def test_nonfinite_rows_stay_in_their_group(dtype, path):
     ends = [70, 75, 140]
     c = case(140, 72, 80, dtype, 4, groups=3)
     at = torch.tensor(ends, dtype=torch.int32, device="cuda")
@@ -251,6 +269,7 @@ def test_float32_modes():
     """Strict float32 is near float64 as a whole as well; the tf32 mode keeps
     16 bits of each operand (parts of 8 and 8: 2^-15 of the magnitudes)."""
     c = case(400, 2048, 264, "float32", 6)
+    before = P.set_kernel_path("tensor-core-pair")
     y = arr(c["x"]).linear(arr(c["w"])).to_torch().double()
     want = c["x"].double() @ c["w"].double()
     assert (y - want).norm() <= 1e-6 * want.norm()
@@ -259,6 +278,7 @@ def test_float32_modes():
         t = arr(c["x"]).linear(arr(c["w"])).to_torch().double()
     finally:
         P.cuda_set_matmul_precision("fp32-strict")
+        P.library().gemm_sm100_set_path(before)
     mag = c["x"].double().abs() @ c["w"].double().abs()
     assert torch.all((t - want).abs() <= (2.0 ** -15 + 2056 * 2.0 ** -23) * mag)
 
@@ -298,6 +318,10 @@ def test_ranks_empty_tensors_and_parts_of_the_gradient():
     y4 = arr(x4).linear(arr(c["w"]), arr(c["bias"]), "relu")
     assert y4.getShape() == [4, 2, 3, 72]
     assert torch.equal(y4.to_torch(), y.view(2, 3, 4, 72).permute(2, 0, 1, 3))
+    res4 = c["res"].view(2, 3, 4, 72).permute(2, 0, 1, 3)      # rows of no single stride
+    y4 = arr(x4).linear(arr(c["w"]), arr(c["bias"]), "relu", arr(res4))
+    y = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]), "relu", arr(c["res"])).to_torch()
+    assert torch.equal(y4.to_torch(), y.view(2, 3, 4, 72).permute(2, 0, 1, 3))
     full = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), arr(c["pre"]), "relu")
     for k, want in enumerate(("inputs", "weights", "bias")):
         only = {n: n == want for n in ("inputs", "weights", "bias")}
@@ -317,8 +341,23 @@ def test_ranks_empty_tensors_and_parts_of_the_gradient():
 
 
 @gpu
+def test_choice_of_kernel():
+    """By the work and the rows, with the name of the last one kept."""
+    def kernel(rows, inner, cols, dtype, layout="plain"):
+        c = case(rows, inner, cols, dtype, 1, layout=layout)
+        arr(c["x"]).linear(arr(c["w"]))
+        return P.cuda_get_backend_info()["kernel"]
+    assert kernel(8, 512, 512, "bfloat16") == "ragged-bf16-128x64"
+    assert kernel(4096, 256, 2048, "float16") == "ragged2-f16-256x256"
+    assert kernel(4096, 1024, 1024, "float32") == "ragged2-bf16x3-256x256"
+    assert kernel(16, 256, 256, "float32") == "ragged-simt-f32"
+    assert kernel(16, 255, 257, "float16") == "ragged-simt-f16"
+
+
+@gpu
+@pytest.mark.parametrize("path", PATHS[1:], indirect=True)
 @pytest.mark.parametrize("dtype", ALL)
-def test_same_bits_again_on_another_stream_and_in_a_graph(dtype):
+def test_same_bits_again_on_another_stream_and_in_a_graph(dtype, path):
     c = case(500, 328, 264, dtype, 15, groups=4)
     ends = torch.tensor([100, 101, 380, 500], dtype=torch.int32, device="cuda")
 
