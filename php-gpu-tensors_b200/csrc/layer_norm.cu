@@ -101,27 +101,26 @@ LayerNormParams params_of(const PtgLayerNorm &a)
 }
 
 // ------------------------------------------------------------ forwards
-// Vectors per thread: 32 elements at most.  With few rows the row is spread
-// over more threads instead (one vector each), which shortens the chain of
-// loads that a launch of a few blocks waits for.
+// Sixteen elements a thread, or 32 where the row is too long for that.  With few
+// rows the row is spread over more threads instead (one vector each), which
+// shortens the chain of loads that a launch of a few blocks waits for.
 template <typename T, int VB>
 cudaError_t forward(const LayerNormParams &p, int sms, cudaStream_t stream)
 {
     constexpr int E = VB / sizeof(T);
-    constexpr int kMost = 32 / E < 16 ? 32 / E : 16;
+    constexpr int kMost = 32 / E, kUsual = 16 / E;
     const long long nvec = p.cols / E;
     if (nvec > static_cast<long long>(kMost) * kMaxThreads) {
         const long long grid = std::min<long long>(p.rows, sms * 8ll);
         return launch(layer_norm_long_kernel<T>, dim3(static_cast<unsigned>(grid)),
                       dim3(kMaxThreads), 0, stream, p);
     }
-    const int want = p.rows <= 4ll * sms ? 1 : std::min(kMost, 4);
-    const int tpr = group_threads(nvec, want);
+    const int tpr = group_threads(nvec, p.rows <= 4ll * sms ? 1 : std::min(kUsual, 8));
     const int nv = static_cast<int>((nvec + tpr - 1) / tpr);
     const dim3 block(tpr, std::max(1, kBlockThreads / tpr));
-    const long long grid = (p.rows + block.y - 1) / block.y;
-    if (grid > 2147483647ll)
-        return cudaErrorInvalidValue;
+    const int threads = static_cast<int>(block.x * block.y);
+    const long long grid = std::min<long long>((p.rows + block.y - 1) / block.y,
+                                               sms * static_cast<long long>(1024 / threads));
     const dim3 g(static_cast<unsigned>(grid));
     if (nv <= 1)
         return launch(layer_norm_kernel<T, VB, 1>, g, block, 0, stream, p);
@@ -132,21 +131,25 @@ cudaError_t forward(const LayerNormParams &p, int sms, cudaStream_t stream)
     if constexpr (kMost > 4) {
         if (nv <= 8)
             return launch(layer_norm_kernel<T, VB, 8>, g, block, 0, stream, p);
-        if constexpr (kMost > 8)
-            return launch(layer_norm_kernel<T, VB, 16>, g, block, 0, stream, p);
+        if constexpr (kMost > 8) {
+            if (nv <= 16)
+                return launch(layer_norm_kernel<T, VB, 16>, g, block, 0, stream, p);
+            if constexpr (kMost > 16)
+                return launch(layer_norm_kernel<T, VB, 32>, g, block, 0, stream, p);
+        }
     }
     return cudaErrorInvalidValue;
 }
 
 // ------------------------------------------------------------ backwards
 template <typename T, int VB, int NV>
-cudaError_t backward_nv(LayerNormParams &p, const PtgLayerNorm &a, int tpr, int sms,
+cudaError_t backward_nv(LayerNormParams &p, const PtgLayerNorm &a, int tpr, const PtgDevice &dev,
                         cudaStream_t stream)
 {
     const dim3 block(tpr, std::max(1, kBlockThreads / tpr));
     const long long need = (p.rows + block.y - 1) / block.y;
     const int grid = static_cast<int>(
-        std::min<long long>(need, std::min(sms * kBackwardBlocksPerSm, kMaxBackwardBlocks)));
+        std::min<long long>(need, std::min(dev.sms * kBackwardBlocksPerSm, kMaxBackwardBlocks)));
     const bool want = a.dgamma || a.dbeta;
     p.partial = want ? a.partial : nullptr;
     const size_t smem = want && block.y > 1 ? static_cast<size_t>(2) * p.cols * 4 : 0;
@@ -162,13 +165,13 @@ cudaError_t backward_nv(LayerNormParams &p, const PtgLayerNorm &a, int tpr, int 
 // Sixteen elements a thread at most: with their gradients' sums and the next
 // row's loads that is what 128 registers hold.
 template <typename T, int VB>
-cudaError_t backward(LayerNormParams &p, const PtgLayerNorm &a, int sms, cudaStream_t stream)
+cudaError_t backward(LayerNormParams &p, const PtgLayerNorm &a, const PtgDevice &dev, cudaStream_t stream)
 {
     constexpr int E = VB / sizeof(T);
     constexpr int kMost = 16 / E;
     const long long nvec = p.cols / E;
     if (nvec > static_cast<long long>(kMost) * kMaxThreads) {
-        const long long grid = std::min<long long>(p.rows, sms * 8ll);
+        const long long grid = std::min<long long>(p.rows, dev.sms * 8ll);
         cudaError_t err = launch(layer_norm_backward_long_kernel<T>,
                                  dim3(static_cast<unsigned>(grid)), dim3(kMaxThreads), 0, stream,
                                  p);
@@ -187,34 +190,35 @@ cudaError_t backward(LayerNormParams &p, const PtgLayerNorm &a, int sms, cudaStr
     const int tpr = group_threads(nvec, kMost);
     const int nv = static_cast<int>((nvec + tpr - 1) / tpr);
     if (nv <= 1)
-        return backward_nv<T, VB, 1>(p, a, tpr, sms, stream);
+        return backward_nv<T, VB, 1>(p, a, tpr, dev, stream);
     if constexpr (kMost > 1)
         if (nv <= 2)
-            return backward_nv<T, VB, 2>(p, a, tpr, sms, stream);
+            return backward_nv<T, VB, 2>(p, a, tpr, dev, stream);
     if constexpr (kMost > 2)
         if (nv <= 4)
-            return backward_nv<T, VB, 4>(p, a, tpr, sms, stream);
+            return backward_nv<T, VB, 4>(p, a, tpr, dev, stream);
     if constexpr (kMost > 4)
         if (nv <= 8)
-            return backward_nv<T, VB, 8>(p, a, tpr, sms, stream);
+            return backward_nv<T, VB, 8>(p, a, tpr, dev, stream);
     if constexpr (kMost > 8)
-        return backward_nv<T, VB, 16>(p, a, tpr, sms, stream);
+        return backward_nv<T, VB, 16>(p, a, tpr, dev, stream);
     return cudaErrorInvalidValue;
 }
 
 template <typename T>
-cudaError_t dispatch(const PtgLayerNorm &a, int sms, bool back, cudaStream_t stream)
+cudaError_t dispatch(const PtgLayerNorm &a, const PtgDevice &dev, bool back,
+                     cudaStream_t stream)
 {
     LayerNormParams p = params_of(a);
     const int vb = vector_bytes(a, sizeof(T));
     if (vb == 16)
-        return back ? backward<T, 16>(p, a, sms, stream) : forward<T, 16>(p, sms, stream);
+        return back ? backward<T, 16>(p, a, dev, stream) : forward<T, 16>(p, dev.sms, stream);
     if (vb == 8)
-        return back ? backward<T, 8>(p, a, sms, stream) : forward<T, 8>(p, sms, stream);
+        return back ? backward<T, 8>(p, a, dev, stream) : forward<T, 8>(p, dev.sms, stream);
     if constexpr (sizeof(T) == 2)
         if (vb == 2)
-            return back ? backward<T, 2>(p, a, sms, stream) : forward<T, 2>(p, sms, stream);
-    return back ? backward<T, 4>(p, a, sms, stream) : forward<T, 4>(p, sms, stream);
+            return back ? backward<T, 2>(p, a, dev, stream) : forward<T, 2>(p, dev.sms, stream);
+    return back ? backward<T, 4>(p, a, dev, stream) : forward<T, 4>(p, dev.sms, stream);
 }
 
 cudaError_t run(const PtgLayerNorm &a, bool back, cudaStream_t stream)
@@ -224,9 +228,9 @@ cudaError_t run(const PtgLayerNorm &a, bool back, cudaStream_t stream)
         return cudaErrorNoDevice;
     cudaError_t err;
     switch (a.dtype) {
-    case DTYPE_FLOAT32: err = dispatch<float>(a, dev.sms, back, stream); break;
-    case DTYPE_FLOAT16: err = dispatch<__half>(a, dev.sms, back, stream); break;
-    case DTYPE_BFLOAT16: err = dispatch<__nv_bfloat16>(a, dev.sms, back, stream); break;
+    case DTYPE_FLOAT32: err = dispatch<float>(a, dev, back, stream); break;
+    case DTYPE_FLOAT16: err = dispatch<__half>(a, dev, back, stream); break;
+    case DTYPE_BFLOAT16: err = dispatch<__nv_bfloat16>(a, dev, back, stream); break;
     default: err = cudaErrorInvalidValue; break;
     }
     if (err == cudaSuccess)

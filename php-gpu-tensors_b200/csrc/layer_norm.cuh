@@ -37,6 +37,7 @@ struct LayerNormParams {
     int gamma_f32, beta_f32;        // parameters held in float32
 };
 
+
 // Sum over the TPR = blockDim.x threads of a row's group; `buf` is a shared
 // array with a place for each warp of the block, a different array for each
 // sum between two barriers.
@@ -60,8 +61,8 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*buf)[32], int t
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++)
-        v[i] = lane < nw ? buf[i][w0 + lane] : 0.0f;
-    for (int o = 16; o > 0; o >>= 1) {
+        v[i] = buf[i][w0 + (lane & (nw - 1))];
+    for (int o = nw >> 1; o > 0; o >>= 1) {
 #pragma unroll
         for (int i = 0; i < N; i++)
             v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
@@ -79,73 +80,143 @@ __device__ __forceinline__ typename RawVec<VB>::type load_row_vec(const T *row, 
     return __ldg(reinterpret_cast<const typename RawVec<VB>::type *>(q));
 }
 
+// A thread's N vectors of the columns it owns (vector v * tpr + t); zeros
+// behind the row.
+template <typename T, int VB, int NV>
+__device__ __forceinline__ void load_owned(const T *row, long long inner, int tpr, int nvec,
+                                           typename RawVec<VB>::type (&raw)[NV])
+{
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int c = v * tpr + static_cast<int>(threadIdx.x);
+        raw[v] = typename RawVec<VB>::type{};
+        if (c < nvec)
+            raw[v] = load_row_vec<T, VB>(row, c, inner);
+    }
+}
+
+// gamma or beta for the owned columns, as pairs; `none` where it is null.
+template <typename T, int VB, int NV, int P>
+__device__ __forceinline__ void load_owned_params(const void *p, int is_f32, float none, int tpr,
+                                                  int nvec, Float2 (&out)[P])
+{
+    constexpr int E = VB / sizeof(T);
+    float v[2 * P];
+#pragma unroll
+    for (int k = 0; k < 2 * P; k++)
+        v[k] = none;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int c = k * tpr + static_cast<int>(threadIdx.x);
+        if (p && c < nvec) {
+            float e[E];
+            load_params<T, E>(p, is_f32, static_cast<long long>(c) * E, e);
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                v[k * E + i] = e[i];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < P; k++)
+        out[k] = pair(v[2 * k], v[2 * k + 1]);
+}
+
+template <typename T, int VB, int NV>
+__device__ __forceinline__ void store_owned(T *row, int tpr, int nvec,
+                                            const typename RawVec<VB>::type (&raw)[NV])
+{
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int c = v * tpr + static_cast<int>(threadIdx.x);
+        if (c < nvec)
+            reinterpret_cast<typename RawVec<VB>::type *>(row)[c] = raw[v];
+    }
+}
+
+template <int P>
+__device__ __forceinline__ float sum_pairs(const Float2 (&v)[P])
+{
+    Float2 s = v[0];
+#pragma unroll
+    for (int k = 1; k < P; k++)
+        s = add2(s, v[k]);
+    float lo, hi;
+    split(s, lo, hi);
+    return lo + hi;
+}
+
+// Forwards: blocks walk the rows with a stride of the grid.  The parameters
+// are read once and the next row's loads are in flight while the current row's
+// two sums are joined.  Arithmetic is on pairs of columns.
 template <typename T, int VB, int NV>
 __global__ void __launch_bounds__(512) layer_norm_kernel(const LayerNormParams p)
 {
     constexpr int E = VB / sizeof(T);
+    constexpr int P = (NV * E + 1) / 2;
+    using Raw = typename RawVec<VB>::type;
     __shared__ float buf[2][1][32];
     grid_dependency_wait();
     grid_launch_dependents();
-    const int tpr = blockDim.x, t = threadIdx.x;
-    const int nvec = p.cols / E;
+    const int tpr = blockDim.x, nvec = p.cols / E;
     const float inv = 1.0f / static_cast<float>(p.cols);
-    const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const bool live = r < p.rows;
-    float x[NV][E];
-    float sum[1] = {0.0f};
-    const T *row = static_cast<const T *>(p.x) + (live ? row_offset(p.xv, r) : 0);
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
+    const long long first = static_cast<long long>(blockIdx.x) * blockDim.y;
+    Raw raw[NV];
+    Float2 gam[P], bet[P];
+    auto fetch = [&](long long r) {
+        if (r < p.rows)
+            load_owned<T, VB, NV>(static_cast<const T *>(p.x) + row_offset(p.xv, r), p.x_inner, tpr,
+                                  nvec, raw);
+    };
+    fetch(first + threadIdx.y);
+    load_owned_params<T, VB, NV>(p.gamma, p.gamma_f32, 1.0f, tpr, nvec, gam);
+    load_owned_params<T, VB, NV>(p.beta, p.beta_f32, 0.0f, tpr, nvec, bet);
+    // every group of the block makes the same number of steps
+    for (long long base = first; base < p.rows; base += step) {
+        const long long r = base + threadIdx.y;
+        Float2 x[P];
+        unpack_pairs<T, VB>(raw, x);
+        fetch(r + step);
+        float sum[1] = {sum_pairs(x)};
+        group_sum(sum, buf[0], tpr);
+        const float mean = sum[0] * inv;
+        const Float2 minus = pair(-mean, -mean);
+        Float2 sq[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-        const int c = v * tpr + t;
-        if (live && c < nvec) {
-            unpack_vec<T, VB>(load_row_vec<T, VB>(row, c, p.x_inner), x[v]);
+        for (int k = 0; k < P; k++)
+            x[k] = add2(x[k], minus);
+        // columns behind the row hold -mean here: they are left out
 #pragma unroll
-            for (int i = 0; i < E; i++)
-                sum[0] += x[v][i];
-        }
-    }
-    group_sum(sum, buf[0], tpr);
-    const float mean = sum[0] * inv;
-    float var[1] = {0.0f};
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-        if (live && v * tpr + t < nvec) {
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                x[v][i] -= mean;
-                var[0] = fmaf(x[v][i], x[v][i], var[0]);
+        for (int k = 0; k < P; k++) {
+            if constexpr (E >= 2) {
+                if ((k / (E / 2)) * tpr + static_cast<int>(threadIdx.x) < nvec)
+                    sq[k & 1] = fma2(x[k], x[k], sq[k & 1]);
+            } else {
+                float lo, hi;
+                split(x[k], lo, hi);
+                lo = 2 * k * tpr + static_cast<int>(threadIdx.x) < nvec ? lo : 0.0f;
+                hi = 2 * k + 1 < NV && (2 * k + 1) * tpr + static_cast<int>(threadIdx.x) < nvec
+                         ? hi : 0.0f;
+                const Float2 q = pair(lo, hi);
+                sq[k & 1] = fma2(q, q, sq[k & 1]);
             }
         }
-    }
-    group_sum(var, buf[1], tpr);
-    if (!live)
-        return;
-    const float rstd = 1.0f / sqrtf(var[0] * inv + p.eps);
-    if (t == 0 && p.mean) {
-        p.mean[r] = mean;
-        p.rstd[r] = rstd;
-    }
-    T *out = static_cast<T *>(p.out) + r * p.cols;
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-        const int c = v * tpr + t;
-        if (c < nvec) {
-            float g[E], b[E];
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                g[i] = 1.0f;
-                b[i] = 0.0f;
-            }
-            if (p.gamma)
-                load_params<T, E>(p.gamma, p.gamma_f32, static_cast<long long>(c) * E, g);
-            if (p.beta)
-                load_params<T, E>(p.beta, p.beta_f32, static_cast<long long>(c) * E, b);
-#pragma unroll
-            for (int i = 0; i < E; i++)
-                x[v][i] = fmaf(x[v][i] * rstd, g[i], b[i]);
-            *reinterpret_cast<typename RawVec<VB>::type *>(out + static_cast<long long>(c) * E) =
-                pack_vec<T, VB>(x[v]);
+        float var[1] = {sum_pairs(sq)};
+        group_sum(var, buf[1], tpr);
+        if (r >= p.rows)
+            continue;
+        const float rstd = 1.0f / sqrtf(var[0] * inv + p.eps);
+        if (threadIdx.x == 0 && p.mean) {
+            p.mean[r] = mean;
+            p.rstd[r] = rstd;
         }
+        const Float2 scale = pair(rstd, rstd);
+#pragma unroll
+        for (int k = 0; k < P; k++)
+            x[k] = fma2(mul2(x[k], scale), gam[k], bet[k]);
+        Raw out[NV];
+        pack_pairs<T, VB>(x, out);
+        store_owned<T, VB, NV>(static_cast<T *>(p.out) + r * p.cols, tpr, nvec, out);
     }
 }
 
@@ -188,93 +259,83 @@ __global__ void __launch_bounds__(512) layer_norm_long_kernel(const LayerNormPar
 }
 
 // Backwards: blocks walk the rows with a stride of the grid; the next row's
-// loads are issued before the current row's sums are joined.
+// loads are issued before the current row's sums are joined.  On pairs of
+// columns, with n = x s - m s and dx = s a - s mean(a) - n s mean(a n), an
+// element costs about seven instructions; in scalar form (and as (x - m) s)
+// issuing them, not memory, was the bound.
 template <typename T, int VB, int NV>
 __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const LayerNormParams p)
 {
     constexpr int E = VB / sizeof(T);
+    constexpr int P = (NV * E + 1) / 2;
     using Raw = typename RawVec<VB>::type;
     __shared__ float buf[2][2][32];
     extern __shared__ float sums[];      // [2][cols] when a block has several groups
     grid_dependency_wait();
     grid_launch_dependents();
-    const int tpr = blockDim.x, t = threadIdx.x;
-    const int nvec = p.cols / E;
+    const int tpr = blockDim.x, nvec = p.cols / E;
     const float inv = 1.0f / static_cast<float>(p.cols);
-    float dg[NV][E], db[NV][E], gam[NV][E];
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            dg[v][i] = db[v][i] = 0.0f;
-            gam[v][i] = 1.0f;
-        }
-        const int c = v * tpr + t;
-        if (p.gamma && c < nvec)
-            load_params<T, E>(p.gamma, p.gamma_f32, static_cast<long long>(c) * E, gam[v]);
-    }
     const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
     const long long first = static_cast<long long>(blockIdx.x) * blockDim.y;
+    const Float2 zero = pair(0.0f, 0.0f);
     Raw rx[NV], rg[NV];
     float mean = 0.0f, rstd = 0.0f;
     auto fetch = [&](long long r) {
-        if (r >= p.rows)
-            return;
-        const T *xr = static_cast<const T *>(p.x) + row_offset(p.xv, r);
-        const T *gr = static_cast<const T *>(p.grad) + row_offset(p.gv, r);
+        if (r < p.rows) {
+            load_owned<T, VB, NV>(static_cast<const T *>(p.x) + row_offset(p.xv, r), p.x_inner, tpr,
+                                  nvec, rx);
+            load_owned<T, VB, NV>(static_cast<const T *>(p.grad) + row_offset(p.gv, r), p.g_inner,
+                                  tpr, nvec, rg);
+            mean = __ldg(p.mean + r);
+            rstd = __ldg(p.rstd + r);
+        } else {                         // adds nothing to any sum
 #pragma unroll
-        for (int v = 0; v < NV; v++) {
-            const int c = v * tpr + t;
-            if (c < nvec) {
-                rx[v] = load_row_vec<T, VB>(xr, c, p.x_inner);
-                rg[v] = load_row_vec<T, VB>(gr, c, p.g_inner);
-            }
+            for (int v = 0; v < NV; v++)
+                rx[v] = rg[v] = Raw{};
+            mean = rstd = 0.0f;
         }
-        mean = __ldg(p.mean + r);
-        rstd = __ldg(p.rstd + r);
     };
     fetch(first + threadIdx.y);
+    Float2 gam[P], dg[P], db[P];
+    load_owned_params<T, VB, NV>(p.gamma, p.gamma_f32, 1.0f, tpr, nvec, gam);
+#pragma unroll
+    for (int k = 0; k < P; k++)
+        dg[k] = db[k] = zero;
     int parity = 0;
     // every group of the block makes the same number of steps
     for (long long base = first; base < p.rows; base += step, parity ^= 1) {
         const long long r = base + threadIdx.y;
-        const bool live = r < p.rows;
-        float n[NV][E], a[NV][E];
-        float s[2] = {0.0f, 0.0f};
-        const float rs = rstd;
-#pragma unroll
-        for (int v = 0; v < NV; v++) {
-            if (live && v * tpr + t < nvec) {
-                unpack_vec<T, VB>(rx[v], n[v]);
-                unpack_vec<T, VB>(rg[v], a[v]);
-#pragma unroll
-                for (int i = 0; i < E; i++) {
-                    n[v][i] = (n[v][i] - mean) * rs;
-                    dg[v][i] = fmaf(a[v][i], n[v][i], dg[v][i]);
-                    db[v][i] += a[v][i];
-                    a[v][i] *= gam[v][i];
-                    s[0] += a[v][i];
-                    s[1] = fmaf(a[v][i], n[v][i], s[1]);
-                }
-            }
-        }
+        const float rs = rstd, shift = -mean * rstd;
+        const Float2 rs2 = pair(rs, rs), shift2 = pair(shift, shift);
+        Float2 n[P], a[P], s0 = zero, s1 = zero;
+        unpack_pairs<T, VB>(rx, n);
+        unpack_pairs<T, VB>(rg, a);
         fetch(r + step);
-        group_sum(s, buf[parity], tpr);
-        if (live) {
-            const float ma = s[0] * inv, mn = s[1] * inv;
-            T *out = static_cast<T *>(p.out) + r * p.cols;
 #pragma unroll
-            for (int v = 0; v < NV; v++) {
-                const int c = v * tpr + t;
-                if (c < nvec) {
-#pragma unroll
-                    for (int i = 0; i < E; i++)
-                        a[v][i] = rs * (a[v][i] - ma - n[v][i] * mn);
-                    *reinterpret_cast<Raw *>(out + static_cast<long long>(c) * E) =
-                        pack_vec<T, VB>(a[v]);
-                }
-            }
+        for (int k = 0; k < P; k++) {
+            n[k] = fma2(n[k], rs2, shift2);
+            dg[k] = fma2(a[k], n[k], dg[k]);
+            db[k] = add2(db[k], a[k]);
+            a[k] = mul2(a[k], gam[k]);
+            s0 = add2(s0, a[k]);
+            s1 = fma2(a[k], n[k], s1);
         }
+        float s[2], hi;
+        split(s0, s[0], hi);
+        s[0] += hi;
+        split(s1, s[1], hi);
+        s[1] += hi;
+        group_sum(s, buf[parity], tpr);
+        if (r >= p.rows)
+            continue;
+        const float c0 = -s[0] * inv * rs, c1 = -s[1] * inv * rs;
+        const Float2 ca = pair(c0, c0), cn = pair(c1, c1);
+#pragma unroll
+        for (int k = 0; k < P; k++)
+            a[k] = fma2(a[k], rs2, fma2(n[k], cn, ca));
+        Raw out[NV];
+        pack_pairs<T, VB>(a, out);
+        store_owned<T, VB, NV>(static_cast<T *>(p.out) + r * p.cols, tpr, nvec, out);
     }
     if (!p.partial)
         return;
@@ -282,15 +343,21 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const LayerNor
     float *dst = blockDim.y > 1 ? sums : part;
     for (int y = 0; y < static_cast<int>(blockDim.y); y++) {
         if (static_cast<int>(threadIdx.y) == y) {
+            float g[2 * P], b[2 * P];
+#pragma unroll
+            for (int q = 0; q < P; q++) {
+                split(dg[q], g[2 * q], g[2 * q + 1]);
+                split(db[q], b[2 * q], b[2 * q + 1]);
+            }
 #pragma unroll
             for (int v = 0; v < NV; v++) {
-                const int c = (v * tpr + t) * E;
-                if (v * tpr + t < nvec) {
+                const int c = (v * tpr + static_cast<int>(threadIdx.x)) * E;
+                if (c < p.cols) {
 #pragma unroll
                     for (int i = 0; i < E; i++) {
-                        dst[c + i] = y == 0 ? dg[v][i] : dst[c + i] + dg[v][i];
-                        dst[p.cols + c + i] =
-                            y == 0 ? db[v][i] : dst[p.cols + c + i] + db[v][i];
+                        const float dgi = g[v * E + i], dbi = b[v * E + i];
+                        dst[c + i] = y == 0 ? dgi : dst[c + i] + dgi;
+                        dst[p.cols + c + i] = y == 0 ? dbi : dst[p.cols + c + i] + dbi;
                     }
                 }
             }
@@ -300,7 +367,7 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const LayerNor
     }
     if (blockDim.y > 1) {
         const int threads = blockDim.x * blockDim.y;
-        for (int c = threadIdx.y * tpr + t; c < 2 * p.cols; c += threads)
+        for (int c = threadIdx.y * tpr + threadIdx.x; c < 2 * p.cols; c += threads)
             part[c] = sums[c];
     }
 }

@@ -108,31 +108,6 @@ bool rows_aligned(const void *p, const RowView &v, int es, int bytes)
     return true;
 }
 
-// Launches the layout pass of `rows` rows of `cols` columns.
-cudaError_t lay_out(int dtype, const void *src, const RowView &v, long long inner, long long rows,
-                    int cols, int parts, void *out, const PtgDevice &dev, cudaStream_t stream)
-{
-    LayParams p;
-    std::memset(&p, 0, sizeof(p));
-    p.src = src;
-    p.rows_of = v;
-    p.inner = inner;
-    p.rows = rows;
-    p.cols = cols;
-    p.ld = static_cast<int>(round8(cols));
-    p.out = static_cast<uint16_t *>(out);
-    p.part = rows * p.ld;
-    p.parts = parts;
-    p.vec = inner == 1 && rows_aligned(src, v, element_bytes(dtype), 16);
-    const long long blocks = (rows * (p.ld / 8) + 255) / 256;
-    if (blocks == 0)
-        return cudaSuccess;
-    const dim3 grid(static_cast<unsigned>(std::min<long long>(blocks, dev.sms * 16ll)));
-    if (dtype == DTYPE_FLOAT32)
-        return launch(lay_out_kernel<float>, grid, 256, 0, stream, p);
-    return launch(lay_out_kernel<__half>, grid, 256, 0, stream, p);   // a copy of 16-bit values
-}
-
 // What a call has decided; `run` is false while it is only being sized.
 struct Plan {
     PtgDevice dev;
@@ -142,6 +117,9 @@ struct Plan {
     cudaError_t err;
     int parts, passes;      // float32: bfloat16 parts and products of them; else 1, 1
     const char *kernel;     // of the last product, for gemm_sm100_last_kernel
+    int dtype;
+    LayParams lay[2];       // layouts that the next product waits for
+    int lays;
 
     bool ok() const { return err == cudaSuccess; }
     void then(cudaError_t e)
@@ -150,6 +128,48 @@ struct Plan {
             err = e;
     }
 };
+
+// Launches the layouts asked for so far.  Blocks for each in proportion to its
+// work, one element vector a thread as far as 16 blocks an SM go.
+void flush_layouts(Plan &pl)
+{
+    if (pl.lays == 0 || !pl.run || !pl.ok())
+        return;
+    auto blocks = [&](const LayParams &p) {
+        const long long n = (p.rows * (p.ld / 8) + 255) / 256;
+        return static_cast<int>(std::min<long long>(n, pl.dev.sms * 16ll));
+    };
+    const int first = blocks(pl.lay[0]), second = pl.lays > 1 ? blocks(pl.lay[1]) : 0;
+    pl.lays = 0;
+    if (first + second == 0)
+        return;
+    if (pl.dtype == DTYPE_FLOAT32)
+        pl.then(launch(lay_out_kernel<float>, dim3(first + second), 256, 0, pl.stream, pl.lay[0],
+                       pl.lay[1], first));
+    else       // a copy of 16-bit values
+        pl.then(launch(lay_out_kernel<__half>, dim3(first + second), 256, 0, pl.stream, pl.lay[0],
+                       pl.lay[1], first));
+}
+
+// Asks for the layout of `rows` rows of `cols` columns.
+void lay_out(Plan &pl, const void *src, const RowView &v, long long inner, long long rows,
+             int cols, void *out)
+{
+    if (pl.lays == 2)
+        flush_layouts(pl);
+    LayParams &p = pl.lay[pl.lays++];
+    std::memset(&p, 0, sizeof(p));
+    p.src = src;
+    p.rows_of = v;
+    p.inner = inner;
+    p.rows = rows;
+    p.cols = cols;
+    p.ld = static_cast<int>(round8(cols));
+    p.out = static_cast<uint16_t *>(out);
+    p.part = rows * p.ld;
+    p.parts = pl.parts;
+    p.vec = inner == 1 && rows_aligned(src, v, element_bytes(pl.dtype), 16);
+}
 
 // Rows as they lie if TMA can read them, else laid out in the workspace.
 Rows plan_rows(Plan &pl, int dtype, const void *p, const RowView &v, long long inner,
@@ -168,7 +188,7 @@ Rows plan_rows(Plan &pl, int dtype, const void *p, const RowView &v, long long i
     void *out = pl.ws.take(static_cast<size_t>(r.part) * pl.parts * 2);
     r.p = out;
     if (pl.run && pl.ok())
-        pl.then(lay_out(dtype, p, v, inner, rows, cols, pl.parts, out, pl.dev, pl.stream));
+        lay_out(pl, p, v, inner, rows, cols, out);
     return r;
 }
 
@@ -217,9 +237,8 @@ Weight plan_weight(Plan &pl, const PtgLinear &a)
     void *out = pl.ws.take(static_cast<size_t>(w.part) * pl.parts * 2);
     w.p = out;
     if (pl.run && pl.ok())
-        pl.then(lay_out(a.dtype, a.w, v, w.cols_contiguous ? a.w_cols : a.w_inner,
-                        static_cast<long long>(a.groups) * rows, cols, pl.parts, out, pl.dev,
-                        pl.stream));
+        lay_out(pl, a.w, v, w.cols_contiguous ? a.w_cols : a.w_inner,
+                static_cast<long long>(a.groups) * rows, cols, out);
     return w;
 }
 
@@ -239,7 +258,7 @@ constexpr int kMaxDevices = 64;
 // CTA pairs of `kernel` that fit the device at one time; raises its
 // shared-memory limit on the first call on a device.  0 on failure.  (The
 // kernel is a template argument: the kernels share one function type.)
-template <auto kernel, int THREADS>
+template <auto kernel>
 int pair_count(int sms)
 {
     static std::mutex mutex;
@@ -261,7 +280,7 @@ int pair_count(int sms)
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(kRaggedThreads);
     cfg.dynamicSmemBytes = kRaggedSmem;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -277,8 +296,7 @@ template <typename T, bool INNER, bool CHUNKED>
 cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p, long long bound)
 {
     constexpr auto kernel = ragged_gemm_kernel<T, INNER, CHUNKED>;
-    constexpr int kThreads = ragged_threads(CHUNKED);
-    const int pairs = pair_count<kernel, kThreads>(pl.dev.sms);
+    const int pairs = pair_count<kernel>(pl.dev.sms);
     if (pairs < 1)
         return cudaErrorInvalidConfiguration;
     p.status = pl.dev.status;
@@ -293,7 +311,7 @@ cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(2 * n));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kRaggedThreads);
     cfg.dynamicSmemBytes = kRaggedSmem;
     cfg.stream = pl.stream;
     cfg.attrs = attr;
@@ -542,6 +560,9 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
                      (path == 1 || few_rows(pl.dev, bound, a.rows, a.groups));
     p.idesc = instruction(a.dtype, p.a_mn, false, few ? 128 : 256);
     pl.kernel = kernel_name(few ? 1 : 0, a.dtype);
+    flush_layouts(pl);
+    if (!pl.ok())
+        return pl.err;
     if (few)
         return a.dtype == DTYPE_FLOAT16 ? launch_decode<__half>(pl, maps, p)
                                         : launch_decode<__nv_bfloat16>(pl, maps, p);
@@ -557,6 +578,9 @@ cudaError_t weight_product(Plan &pl, const PtgLinear &a, const Rows &x, const Ro
                            CUtensorMap *group_maps)
 {
     pl.kernel = kernel_name(0, a.dtype);
+    flush_layouts(pl);
+    if (!pl.ok())
+        return pl.err;
     RaggedParams p;
     std::memset(&p, 0, sizeof(p));
     p.ends = a.ends;
@@ -605,6 +629,7 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
     std::memset(&pl, 0, sizeof(pl));
     pl.err = cudaSuccess;
     pl.stream = stream;
+    pl.dtype = a.dtype;
     pl.run = run;
     if (run && a.workspace)
         pl.ws.base = reinterpret_cast<uint8_t *>(
@@ -620,7 +645,7 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
 // multiply-adds, 16-bit ones below kSimtLayWork whose operands would have to
 // be laid out first.  The thread's kernel path decides first (2: CUDA cores,
 // 1 and 3: the tensor-core kernels).
-constexpr double kSimtWork = 1.0e9;
+constexpr double kSimtWork = 5.0e8;
 constexpr double kSimtLayWork = 5.0e7;
 
 bool on_cuda_cores(const PtgLinear &a, bool lay)
@@ -759,13 +784,15 @@ void backward(Plan &pl, const PtgLinear &a)
         }
         return;
     }
-    if (a.dx) {
-        const Weight w = plan_weight(pl, a);
-        if (pl.run && pl.ok())
-            pl.then(product(pl, a, dz, w, true, p));
-    }
+    Weight w;
+    Rows x;
+    if (a.dx)
+        w = plan_weight(pl, a);
+    if (a.dw)
+        x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
+    if (a.dx && pl.run && pl.ok())
+        pl.then(product(pl, a, dz, w, true, p));
     if (a.dw) {
-        const Rows x = plan_rows(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
         CUtensorMap *maps = nullptr;
         if (a.ends)
             maps = static_cast<CUtensorMap *>(pl.ws.take(sizeof(CUtensorMap) * 2 * a.groups));

@@ -59,23 +59,42 @@ __device__ __forceinline__ void load8(const T *row, long long inner, int c, int 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) lay_out_kernel(const LayParams p)
+__device__ __forceinline__ void lay_out_one(const LayParams &p, long long r, int c)
+{
+    const T *row = static_cast<const T *>(p.src) + row_offset(p.rows_of, r);
+    alignas(16) T v[8];
+    load8(row, p.inner, c, p.cols, p.vec, v);
+    uint16_t *out = p.out + r * p.ld + c;
+    if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(v);
+    else
+        store_parts(v, out, p.part, p.parts);
+}
+
+// One or two layouts in a launch: blocks below `first` make a, the others b.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    lay_out_kernel(const LayParams a, const LayParams b, const int first)
 {
     grid_dependency_wait();
     grid_launch_dependents();
+    const bool second = static_cast<int>(blockIdx.x) >= first;
+    const LayParams &p = second ? b : a;
+    const int block = second ? blockIdx.x - first : blockIdx.x;
+    const int blocks = second ? gridDim.x - first : first;
     const int per_row = p.ld / 8;
     const long long total = p.rows * per_row;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const long long r = i / per_row;
-        const int c = static_cast<int>(i - r * per_row) * 8;
-        const T *row = static_cast<const T *>(p.src) + row_offset(p.rows_of, r);
-        alignas(16) T v[8];
-        load8(row, p.inner, c, p.cols, p.vec, v);
-        uint16_t *out = p.out + r * p.ld + c;
-        if constexpr (sizeof(T) == 2)
-            *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(v);
-        else
-            store_parts(v, out, p.part, p.parts);
+    if (total < (1ll << 31)) {
+        const unsigned n = static_cast<unsigned>(total), step = blocks * 256u;
+        for (unsigned i = block * 256u + threadIdx.x; i < n; i += step) {
+            const unsigned r = i / per_row;
+            lay_out_one<T>(p, r, static_cast<int>(i - r * per_row) * 8);
+        }
+    } else {
+        for (long long i = block * 256ll + threadIdx.x; i < total; i += blocks * 256ll) {
+            const long long r = i / per_row;
+            lay_out_one<T>(p, r, static_cast<int>(i - r * per_row) * 8);
+        }
     }
 }
 
@@ -119,14 +138,15 @@ struct SlopeParams {
     int strips;             // column strips: block = row tile * strips + strip
 };
 
-// Rows r0 + lane_y + 8 k of one block, four at a time: all their loads are in
-// flight before the first is used.
+// Rows r0 + lane_y + 8 k of one block, kBatch at a time: all their loads are in
+// flight before the first is used (64 registers, so that four blocks share an
+// SM: 64 KB of loads).
 template <typename T, int ACT>
 __device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1, int c, int lane_y,
                                            float (&sum)[8])
 {
     constexpr bool kFast = sizeof(T) == 2;
-    constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;
+    constexpr int kBatch = sizeof(T) == 2 ? 2 : 1;
 #pragma unroll 1
     for (int base = r0 + lane_y; base < r1; base += 8 * kBatch) {
         alignas(16) T g[kBatch][8], z[kBatch][8];
@@ -152,10 +172,15 @@ __device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1,
                 v[i] = to_float(g[k][i]);
                 if constexpr (ACT != CUDA_MATMUL_EPILOGUE_NONE)
                     v[i] *= activation_slope<ACT, kFast>(to_float(z[k][i]));
-                if (c + i >= p.cols)
-                    v[i] = 0.0f;
-                sum[i] += v[i];
             }
+            if (c + 8 > p.cols) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    v[i] = c + i < p.cols ? v[i] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                sum[i] += v[i];
             if (p.dz) {
                 uint16_t *out =
                     static_cast<uint16_t *>(p.dz) + static_cast<long long>(r) * p.ld + c;
@@ -174,7 +199,7 @@ __device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p)
+__global__ void __launch_bounds__(256, 4) slope_kernel(const SlopeParams p)
 {
     __shared__ float acc[8][kSlopeCols + 8];
     extern __shared__ int table[];

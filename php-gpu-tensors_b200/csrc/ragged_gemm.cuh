@@ -68,11 +68,10 @@ struct RaggedMaps {
 constexpr int kMaxGroups = 2048;
 constexpr int kRaggedBN = 256;
 constexpr int kRaggedStages = 6;
-// Epilogue warps: 16 hide each other's latencies (TMEM, residual, stores);
-// CHUNKED ones keep a tile's sums in registers, which eight warps have room
-// for.
-constexpr int ragged_epi_warps(bool chunked) { return chunked ? 8 : 16; }
-constexpr int ragged_threads(bool chunked) { return 32 * (2 + ragged_epi_warps(chunked)); }
+// Sixteen epilogue warps hide each other's latencies (TMEM, residual, stores);
+// CHUNKED ones keep a tile's sums in registers, 64 each.
+constexpr int kRaggedEpiWarps = 16;
+constexpr int kRaggedThreads = 32 * (2 + kRaggedEpiWarps);
 constexpr int kRaggedTile = 16384;                       // 128 rows x 64 of K, 16 bits
 constexpr int kRaggedRing = kRaggedStages * 2 * kRaggedTile;
 constexpr int kRaggedBars = 2 * kRaggedStages + 4 + 1;
@@ -347,11 +346,11 @@ __global__ void __launch_bounds__(256)
 }
 
 template <typename T, bool INNER, bool CHUNKED>
-__global__ void __launch_bounds__(ragged_threads(CHUNKED), 1)
+__global__ void __launch_bounds__(kRaggedThreads, 1)
     ragged_gemm_kernel(const __grid_constant__ RaggedMaps maps, const RaggedParams p)
 {
     constexpr int S = kRaggedStages;
-    constexpr int kEpiWarps = ragged_epi_warps(CHUNKED);
+    constexpr int kEpiWarps = kRaggedEpiWarps;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -573,7 +572,7 @@ __global__ void __launch_bounds__(ragged_threads(CHUNKED), 1)
             T res[kGroup];
             if constexpr (!INNER) {
                 bias = load_bias<T>(p, r.group, feature);
-                if (p.residual && mine > 0)      // in flight while the products run
+                if (!CHUNKED && p.residual && mine > 0)      // in flight while the products run
                     load_residual(p, n0, r.n_end - n0, feature, res);
             }
             const int chunks =
@@ -600,20 +599,20 @@ __global__ void __launch_bounds__(ragged_threads(CHUNKED), 1)
                 if constexpr (CHUNKED) {
                     if (chunks > 1) {
 #pragma unroll
-                        for (int h = 0; h < kCols / 32; h++) {
-                            if (h * 32 < mine) {
-                                uint32_t raw[32];
-                                tmem_ld_32x32b_x32(t_acc + h * 32, raw);
-                                tmem_ld_wait();
+                        for (int h = 0; h < kCols / 16; h++) {
+                            if (h * 16 < mine) {
+                                uint32_t raw[16];
+                                tmem_ld_32x32b_x16(t_acc + h * 16, raw);
+                                tmem_ld_wait_regs(raw);
 #pragma unroll
-                                for (int j = 0; j < 32; j++)
-                                    total[h * 32 + j] += __uint_as_float(raw[j]);
+                                for (int j = 0; j < 16; j++)
+                                    total[h * 16 + j] += __uint_as_float(raw[j]);
                                 if (c == chunks - 1) {
                                     // the sums take the last chunk's place
 #pragma unroll
-                                    for (int j = 0; j < 32; j++)
-                                        raw[j] = __float_as_uint(total[h * 32 + j]);
-                                    tmem_st_32x32b_x32(t_acc + h * 32, raw);
+                                    for (int j = 0; j < 16; j++)
+                                        raw[j] = __float_as_uint(total[h * 16 + j]);
+                                    tmem_st_32x32b_x16(t_acc + h * 16, raw);
                                 }
                             }
                         }
@@ -621,9 +620,14 @@ __global__ void __launch_bounds__(ragged_threads(CHUNKED), 1)
                     }
                 }
                 if (c == chunks - 1) {
-uint32_t raw[kGroup];
-                    if (mine > 0)
+                    uint32_t raw[kGroup];
+                    if (mine > 0) {
                         tmem_ld_32x32b_x16(t_acc, raw);
+                        if constexpr (CHUNKED && !INNER) {   // (the sums took the registers)
+                            if (p.residual)
+                                load_residual(p, n0, r.n_end - n0, feature, res);
+                        }
+                    }
 #pragma unroll 1
                     for (int h = 0; h < mine; h += kGroup) {
                         float v[kGroup];

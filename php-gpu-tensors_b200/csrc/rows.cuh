@@ -103,4 +103,83 @@ __device__ __forceinline__ void load_params(const void *p, int is_f32, long long
     }
 }
 
+// Two floats in one 64-bit register pair, and the packed arithmetic of sm_100
+// (one instruction for both, each rounded as its scalar form).
+struct Float2 {
+    unsigned long long v;
+};
+
+__device__ __forceinline__ Float2 pair(float lo, float hi)
+{
+    Float2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ void split(Float2 a, float &lo, float &hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+
+__device__ __forceinline__ Float2 add2(Float2 a, Float2 b)
+{
+    Float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+__device__ __forceinline__ Float2 mul2(Float2 a, Float2 b)
+{
+    Float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+__device__ __forceinline__ Float2 fma2(Float2 a, Float2 b, Float2 c)
+{
+    Float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// N raw vectors of a thread as pairs, and back.
+template <typename T, int VB, int N, int P>
+__device__ __forceinline__ void unpack_pairs(const typename RawVec<VB>::type (&raw)[N],
+                                             Float2 (&out)[P])
+{
+    constexpr int E = VB / sizeof(T);
+    float v[2 * P];
+    v[2 * P - 1] = 0.0f;             // a lone element's partner
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        float e[E];
+        unpack_vec<T, VB>(raw[k], e);
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            v[k * E + i] = e[i];
+    }
+#pragma unroll
+    for (int k = 0; k < P; k++)
+        out[k] = pair(v[2 * k], v[2 * k + 1]);
+}
+
+template <typename T, int VB, int N, int P>
+__device__ __forceinline__ void pack_pairs(const Float2 (&in)[P],
+                                           typename RawVec<VB>::type (&raw)[N])
+{
+    constexpr int E = VB / sizeof(T);
+    float v[2 * P];
+#pragma unroll
+    for (int k = 0; k < P; k++)
+        split(in[k], v[2 * k], v[2 * k + 1]);
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        float e[E];
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            e[i] = v[k * E + i];
+        raw[k] = pack_vec<T, VB>(e);
+    }
+}
+
 } // namespace ptg

@@ -424,11 +424,12 @@ class CudaArray:
         [cols] arrays of this dtype or float32.  With save_stats the result is
         (y, mean, rstd), the float32 statistics layer_norm_backward takes."""
         _check_feed_forward("layer_norm", self, gamma, beta)
-        y = _result(self._shape, self._dtype)
+        y = _result(self._shape, self._dtype, self)
         lead = self._shape[:-1]
         mean = rstd = None
         if save_stats:
-            mean, rstd = _result(lead, "float32"), _result(lead, "float32")
+            mean = _result(lead, "float32")
+            rstd = _result(lead, "float32", mean)
         _raise_for(library().pt_layer_norm(
             _ref(self), _ref(gamma), _ref(beta), eps, _ref(y), _ptr(mean), _ptr(rstd),
             _raw_stream()))
@@ -478,13 +479,16 @@ def _check_feed_forward(what, *arrays):
             raise InvalidArgumentException("%s operands must be CudaArrays" % what)
 
 
-def _result(shape, dtype):
-    """An uninitialised contiguous array."""
-    torch = _torch()
+def _result(shape, dtype, like=None):
+    """An uninitialised contiguous array; `like`, an array of the same type,
+    saves torch's own argument handling."""
     self = CudaArray.__new__(CudaArray)
-    self._dtype, self._flat, self._offset = dtype, None, 0
-    self._tensor = torch.empty(shape, dtype=_TORCH_DTYPES[dtype], device="cuda")
-    self._shape, self._strides = list(shape), _contiguous_strides(shape)
+    if like is not None and like._tensor is not None:
+        t = like._tensor.new_empty(shape)
+    else:
+        t = _torch().empty(shape, dtype=_TORCH_DTYPES[dtype], device="cuda")
+    self._tensor, self._flat, self._dtype, self._offset = t, None, dtype, 0
+    self._shape, self._strides = list(shape), list(t.stride())
     return self
 
 
@@ -517,12 +521,13 @@ def layer_norm_backward(grad, x, gamma, mean, rstd, params=True):
         if s._dtype != "float32" or s._shape != lead or s._strides != _contiguous_strides(lead):
             raise InvalidArgumentException(
                 "layer norm statistics must be contiguous float32 arrays, one value a row")
-    dx = _result(x._shape, x._dtype)
+    dx = _result(x._shape, x._dtype, x)
     dgamma = dbeta = work = None
     lib = library()
     size = ctypes.c_size_t(0)
     if params:
-        dgamma, dbeta = _result([cols], "float32"), _result([cols], "float32")
+        dgamma = _result([cols], "float32", mean)
+        dbeta = _result([cols], "float32", mean)
         size.value = lib.pt_layer_norm_backward_workspace(math.prod(lead), cols)
         work = _workspace(size.value)
     _raise_for(lib.pt_layer_norm_backward(
@@ -549,15 +554,16 @@ def _check_ends(ends, weight):
     return ends.data_ptr()
 
 
-def _with_workspace(call):
-    """Runs call(workspace, size) and, where it asks for a workspace, again
-    with one."""
+def _with_workspace(call, args, stream):
+    """call(*args, workspace, size, stream), and where it asks for a workspace
+    again with one."""
     size = ctypes.c_size_t(0)
-    status = call(None, ctypes.addressof(size))
+    status = call(*args, None, ctypes.addressof(size), stream)
     if status == PT_WORKSPACE:
         work = _workspace(size.value)
-        status = call(work.data_ptr(), ctypes.addressof(size))
-    _raise_for(status)
+        status = call(*args, work.data_ptr(), ctypes.addressof(size), stream)
+    if status != PT_OK:
+        _raise_for(status)
 
 
 def _linear(x, weight, ends, bias, activation, residual, save_pre):
@@ -566,11 +572,11 @@ def _linear(x, weight, ends, bias, activation, residual, save_pre):
         raise InvalidArgumentException("linear layers require rows and a weight")
     code = _activation_code(activation)
     shape = x._shape[:-1] + weight._shape[-1:]
-    y = _result(shape, x._dtype)
-    pre = _result(shape, x._dtype) if save_pre else None
-    args = (_ref(x), _ref(weight), ends, _ref(bias), code, _ref(residual), _ref(y), _ref(pre))
-    stream, lib = _raw_stream(), library()
-    _with_workspace(lambda work, size: lib.pt_linear(*args, work, size, stream))
+    y = _result(shape, x._dtype, x)
+    pre = _result(shape, x._dtype, x) if save_pre else None
+    _with_workspace(library().pt_linear,
+                    (_ref(x), _ref(weight), ends, _ref(bias), code, _ref(residual), _ref(y),
+                     _ref(pre)), _raw_stream())
     return (y, pre) if save_pre else y
 
 
@@ -578,13 +584,15 @@ def _linear_backward(grad, x, weight, ends, pre, activation, bias, inputs, weigh
                      weight_grad_dtype):
     _check_feed_forward("linear_backward", grad, x, weight, pre)
     code = _activation_code(activation)
-    dx = _result(x._shape, x._dtype) if inputs else None
-    dw = _result(weight._shape, weight_grad_dtype or x._dtype) if weights else None
+    dx = _result(x._shape, x._dtype, x) if inputs else None
+    dw = None
+    if weights:
+        dw = _result(weight._shape, weight_grad_dtype or x._dtype,
+                     None if weight_grad_dtype else x)
     dbias = _result(weight._shape[:-2] + weight._shape[-1:], "float32") if bias else None
-    args = (_ref(grad), _ref(x), _ref(weight), ends, _ref(pre), code, _ref(dx), _ref(dw),
-            _ptr(dbias))
-    stream, lib = _raw_stream(), library()
-    _with_workspace(lambda work, size: lib.pt_linear_backward(*args, work, size, stream))
+    _with_workspace(library().pt_linear_backward,
+                    (_ref(grad), _ref(x), _ref(weight), ends, _ref(pre), code, _ref(dx), _ref(dw),
+                     _ptr(dbias)), _raw_stream())
     return dx, dw, dbias
 
 
