@@ -416,9 +416,12 @@ def test_refusals():
                 None) == P.PT_INVALID_ARGUMENT            # an activation without pre
     assert back(ref(y), ref(x), ref(w), None, None, 0, ref(x), ref(_pt([8, 16], "bfloat16")), None,
                 None, ref(size), None) == P.PT_INVALID_ARGUMENT
-    # float32 operands need a place for their parts, and say how large
+    # float32 operands on the tensor cores need a place for their parts, and say
+    # how large
     x, w, y = _pt([4, 8], "float32"), _pt([8, 16], "float32"), _pt([4, 16], "float32")
+    before = P.set_kernel_path("tensor-core-pair")
     assert forward(x=x, w=w, y=y) == P.PT_WORKSPACE
+    lib.gemm_sm100_set_path(before)
     assert size.value >= 3 * 2 * (4 * 8 + 8 * 16)
     with pytest.raises(P.InvalidArgumentException):
         P._activation_code("swish")
