@@ -58,12 +58,14 @@ cudaError_t launch(Kernel kernel, dim3 grid, int block, size_t smem, cudaStream_
 // A rank-5 tiled map; strides in elements of `es` bytes, axes past `rank`
 // have extent 1.
 bool encode(const PtgDevice &dev, CUtensorMap *map, int dtype, const void *base, int rank,
-            const long long *ext, const long long *stride, int box0, int box1)
+            const long long *ext, const long long *stride, int box0, int box1, int box2 = 1,
+            bool swizzled = true)
 {
     if (!dev.encode)
         return false;
     cuuint64_t dims[5], strides[4];
-    cuuint32_t box[5] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(box1), 1, 1, 1};
+    cuuint32_t box[5] = {static_cast<cuuint32_t>(box0), static_cast<cuuint32_t>(box1),
+                         static_cast<cuuint32_t>(box2), 1, 1};
     cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     const cuuint64_t filler = static_cast<cuuint64_t>(round8(ext[0])) * 2;
     for (int i = 0; i < 5; i++) {
@@ -75,7 +77,8 @@ bool encode(const PtgDevice &dev, CUtensorMap *map, int dtype, const void *base,
                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(dev.encode)(
                map, type, 5, const_cast<void *>(base), dims, strides, box, steps,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_INTERLEAVE_NONE,
+               swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
            CUDA_SUCCESS;
 }
@@ -527,6 +530,20 @@ Plain plan_plain(Plan &pl, int dtype, const void *src, const RowView &v, long lo
 }
 
 // ------------------------------------------------------------ tensor cores
+// Maps of a 16-bit result (and of pre), where TMA can store to them.
+void result_maps(const Plan &pl, int dtype, RaggedParams &p, RaggedMaps &maps, long long rows,
+                 int groups)
+{
+    if (dtype == DTYPE_FLOAT32 || p.features % 8 != 0 || !aligned(p.out, 16) ||
+        (p.pre && !aligned(p.pre, 16)))
+        return;
+    const long long ext[3] = {p.features, rows, groups};
+    const long long str[3] = {1, p.out_row, p.out_group};
+    p.tma_store =
+        encode(pl.dev, &maps.out, dtype, p.out, 3, ext, str, 32, kGroup, 1, false) &&
+        (!p.pre || encode(pl.dev, &maps.pre, dtype, p.pre, 3, ext, str, 32, kGroup, 1, false));
+}
+
 // Rows x weight: `features` columns of the result, `inner` summed over.
 // transposed: the weight's inner axis gives the features (dx).
 cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w,
@@ -543,18 +560,33 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
     p.out_row = features;
     RaggedMaps maps;
     std::memset(&maps, 0, sizeof(maps));
-    const long long wext[4] = {p.a_mn ? features : inner, p.a_mn ? inner : features, a.groups,
-                               pl.parts};
-    const long long wstr[4] = {1, w.ld, w.group, w.part};
+    p.a_chunks = p.a_mn && features % 64 == 0;
+    const long long wext[5] = {p.a_chunks ? 64 : p.a_mn ? features : inner,
+                               p.a_mn ? inner : features,
+                               p.a_chunks ? features / 64 : a.groups,
+                               p.a_chunks ? a.groups : pl.parts, pl.parts};
+    const long long wstr[5] = {1, w.ld, p.a_chunks ? 64 : w.group, p.a_chunks ? w.group : w.part,
+                               w.part};
     const long long xext[3] = {inner, a.rows, pl.parts};
     const long long xstr[3] = {1, x.ld, x.part};
-    if (inner > 0 &&
-        (!encode(pl.dev, &maps.a, a.dtype, w.p, 4, wext, wstr, 64, p.a_mn ? 64 : 128) ||
-         !encode(pl.dev, &maps.b, a.dtype, x.p, 3, xext, xstr, 64, 128) ||
-         !encode(pl.dev, &maps.b16, a.dtype, x.p, 3, xext, xstr, 64, 16)))
-        return cudaErrorInvalidValue;
-    const long long bound = static_cast<long long>((features + 255) / 256) *
-                            (a.rows / kRaggedBN + std::min(a.groups, a.rows));
+    if (inner > 0) {
+        bool ok = encode(pl.dev, &maps.a, a.dtype, w.p, p.a_chunks ? 5 : 4, wext, wstr, 64,
+                         p.a_mn ? 64 : 128, p.a_chunks ? 2 : 1);
+        for (int i = 0; i < 4; i++)
+            ok = ok && encode(pl.dev, &maps.rows[i], a.dtype, x.p, 3, xext, xstr, 64, 16 << i);
+        if (!ok)
+            return cudaErrorInvalidValue;
+    }
+    p.split = 1;
+    const long long ft = (features + 255) / 256;
+    auto row_tiles = [&](int span) {
+        return a.ends ? a.rows / span + std::min(a.groups, a.rows)
+                      : static_cast<long long>((a.rows + span - 1) / span);
+    };
+    // tiles of fewer rows while the pairs are not all at work: they load more
+    // of the weight per row, but an idle pair loads nothing
+    p.span = kRaggedBN;
+    long long bound = ft * row_tiles(p.span);
     const int path = ptg_path();
     const bool few = a.dtype != DTYPE_FLOAT32 && path != 3 &&
                      (path == 1 || few_rows(pl.dev, bound, a.rows, a.groups));
@@ -563,9 +595,14 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
     flush_layouts(pl);
     if (!pl.ok())
         return pl.err;
+    while (p.span > 64 && ft * row_tiles(p.span / 2) <= pl.dev.sms / 2) {
+        p.span /= 2;
+        bound = ft * row_tiles(p.span);
+    }
     if (few)
         return a.dtype == DTYPE_FLOAT16 ? launch_decode<__half>(pl, maps, p)
                                         : launch_decode<__nv_bfloat16>(pl, maps, p);
+    result_maps(pl, a.dtype, p, maps, a.rows, 1);
     switch (a.dtype) {
     case DTYPE_FLOAT16: return launch_pairs<__half, false, false>(pl, maps, p, bound);
     case DTYPE_BFLOAT16: return launch_pairs<__nv_bfloat16, false, false>(pl, maps, p, bound);
@@ -573,9 +610,23 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
     }
 }
 
-// dw[g] = sum over the rows of group g of x^T dz.
+// Parts that the rows of a group are cut into for dw: while its tiles leave
+// pairs idle, and every part keeps eight k-blocks on average.  A rule of the
+// sizes alone, since it also sizes the workspace.
+constexpr int kPairs = 74;
+
+int weight_parts(const PtgLinear &a)
+{
+    const long long tiles = static_cast<long long>((a.cols + 255) / 256) *
+                            ((a.inner + kRaggedBN - 1) / kRaggedBN) * a.groups;
+    const long long blocks = a.rows / a.groups / 64;
+    return static_cast<int>(std::max<long long>(1, std::min(kPairs / tiles, blocks / 8)));
+}
+
+// dw[g] = sum over the rows of group g of x^T dz.  With several parts each
+// writes its float32 sums to `partial`, and add_parts_kernel joins them.
 cudaError_t weight_product(Plan &pl, const PtgLinear &a, const Rows &x, const Rows &dz,
-                           CUtensorMap *group_maps)
+                           CUtensorMap *group_maps, int parts, float *partial)
 {
     pl.kernel = kernel_name(0, a.dtype);
     flush_layouts(pl);
@@ -589,39 +640,62 @@ cudaError_t weight_product(Plan &pl, const PtgLinear &a, const Rows &x, const Ro
     p.features = a.cols;
     p.cols = a.inner;
     p.passes = pl.passes;
+    p.span = kRaggedBN;
+    p.split = parts;
     p.idesc = instruction(a.dtype, true, true, 256);
-    p.out = a.dw;
+    p.out = parts > 1 ? partial : a.dw;
     p.out_row = a.cols;
     p.out_group = static_cast<long long>(a.inner) * a.cols;
+    p.out_part = p.out_group * a.groups;
     RaggedMaps maps;
     std::memset(&maps, 0, sizeof(maps));
-    auto rows_map = [&](CUtensorMap *map, const Rows &m, int cols) {
-        const long long ext[3] = {cols, a.rows, pl.parts};
-        const long long str[3] = {1, m.ld, m.part};
-        return encode(pl.dev, map, a.dtype, m.p, 3, ext, str, 64, 64);
+    auto rows_map = [&](CUtensorMap *map, const Rows &m, int cols, int chunks) {
+        const long long ext[4] = {chunks ? 64 : cols, a.rows, chunks ? cols / 64 : pl.parts,
+                                  pl.parts};
+        const long long str[4] = {1, m.ld, chunks ? 64 : m.part, m.part};
+        return encode(pl.dev, map, a.dtype, m.p, chunks ? 4 : 3, ext, str, 64, 64, chunks ? 2 : 1);
     };
-    if (!rows_map(&maps.a, dz, a.cols) || !rows_map(&maps.b, x, a.inner))
+    p.a_chunks = a.cols % 64 == 0;
+    p.b_chunks = a.inner % 64 == 0;
+    if (!rows_map(&maps.a, dz, a.cols, p.a_chunks) || !rows_map(&maps.b, x, a.inner, p.b_chunks))
         return cudaErrorInvalidValue;
+    cudaError_t err = cudaSuccess;
     if (a.ends) {
         p.group_maps = group_maps;
-        const cudaError_t err =
-            launch(group_maps_kernel, dim3(1), 256, static_cast<size_t>(a.groups) * 8, pl.stream,
-                   maps.a, maps.b, a.ends, a.groups, a.rows, group_maps);
+        err = launch(group_maps_kernel, dim3(1), 256, static_cast<size_t>(a.groups) * 8, pl.stream,
+                     maps.a, maps.b, a.ends, a.groups, a.rows, group_maps);
         if (err != cudaSuccess)
             return err;
     }
     const long long bound = static_cast<long long>((a.cols + 255) / 256) *
-                            ((a.inner + kRaggedBN - 1) / kRaggedBN) * a.groups;
+                            ((a.inner + kRaggedBN - 1) / kRaggedBN) * a.groups * parts;
+    const int out_dtype = parts > 1 ? static_cast<int>(DTYPE_FLOAT32) : a.dw_dtype;
+    result_maps(pl, out_dtype, p, maps, a.inner, a.groups);
     if (a.dtype == DTYPE_FLOAT32)
-        return launch_pairs<float, true, true>(pl, maps, p, bound);
-    if (a.dtype == DTYPE_FLOAT16) {
-        if (a.dw_dtype == DTYPE_FLOAT32)
-            return launch_pairs<float, true, false>(pl, maps, p, bound);
-        return launch_pairs<__half, true, false>(pl, maps, p, bound);
-    }
+        err = launch_pairs<float, true, true>(pl, maps, p, bound);
+    else if (out_dtype == DTYPE_FLOAT32)
+        err = launch_pairs<float, true, false>(pl, maps, p, bound);
+    else if (a.dtype == DTYPE_FLOAT16)
+        err = launch_pairs<__half, true, false>(pl, maps, p, bound);
+    else
+        err = launch_pairs<__nv_bfloat16, true, false>(pl, maps, p, bound);
+    if (err != cudaSuccess || parts == 1)
+        return err;
+    const long long n = p.out_part;
+    const int vec = n % 4 == 0 && aligned(a.dw, 16);
+    const dim3 grid(static_cast<unsigned>(
+        std::min<long long>((n + 1023) / 1024, pl.dev.sms * 16ll)));
     if (a.dw_dtype == DTYPE_FLOAT32)
-        return launch_pairs<float, true, false>(pl, maps, p, bound);
-    return launch_pairs<__nv_bfloat16, true, false>(pl, maps, p, bound);
+        return launch(add_parts_kernel<float>, grid, 256, 0, pl.stream,
+                      static_cast<const float *>(partial), parts, n, n, vec,
+                      static_cast<float *>(a.dw));
+    if (a.dw_dtype == DTYPE_FLOAT16)
+        return launch(add_parts_kernel<__half>, grid, 256, 0, pl.stream,
+                      static_cast<const float *>(partial), parts, n, n, vec,
+                      static_cast<__half *>(a.dw));
+    return launch(add_parts_kernel<__nv_bfloat16>, grid, 256, 0, pl.stream,
+                  static_cast<const float *>(partial), parts, n, n, vec,
+                  static_cast<__nv_bfloat16 *>(a.dw));
 }
 
 bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
@@ -682,6 +756,9 @@ void forward(Plan &pl, const PtgLinear &a)
         p.residual = r.p;
         p.residual_row = r.row;
         p.residual_inner = r.inner;
+        p.residual_small = static_cast<double>(a.rows) * std::max(1ll, r.row) +
+                               static_cast<double>(a.cols) * r.inner <
+                           2147483648.0 / element_bytes(a.dtype);
     }
     if (on_cuda_cores(a, needs_layout(a, a.x, a.xv, a.x_inner, a.inner))) {
         const Plain x = plan_plain(pl, a.dtype, a.x, a.xv, a.x_inner, a.rows, a.inner);
@@ -796,8 +873,13 @@ void backward(Plan &pl, const PtgLinear &a)
         CUtensorMap *maps = nullptr;
         if (a.ends)
             maps = static_cast<CUtensorMap *>(pl.ws.take(sizeof(CUtensorMap) * 2 * a.groups));
+        const int parts = weight_parts(a);
+        float *part = nullptr;
+        if (parts > 1)
+            part = static_cast<float *>(pl.ws.take(static_cast<size_t>(parts) * a.groups *
+                                                   a.inner * a.cols * 4));
         if (pl.run && pl.ok())
-            pl.then(weight_product(pl, a, x, dz, maps));
+            pl.then(weight_product(pl, a, x, dz, maps, parts, part));
     }
 }
 

@@ -112,6 +112,40 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const T *src, const RowV
     }
 }
 
+// out[i] = the parts' float32 results at i, added in order and rounded once.
+// n is a multiple of 4 elements or vec is 0.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, int count,
+                                                        long long stride, long long n, int vec,
+                                                        T *out)
+{
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const long long step = gridDim.x * 256ll;
+    if (vec) {
+        for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n / 4; i += step) {
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k = 0; k < count; k++) {
+                const float4 q = *reinterpret_cast<const float4 *>(parts + k * stride + i * 4);
+                sum.x += q.x;
+                sum.y += q.y;
+                sum.z += q.z;
+                sum.w += q.w;
+            }
+            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+            constexpr int VB = 4 * static_cast<int>(sizeof(T));
+            reinterpret_cast<typename RawVec<VB>::type *>(out)[i] = pack_vec<T, VB>(v);
+        }
+    } else {
+        for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += step) {
+            float sum = 0.0f;
+            for (int k = 0; k < count; k++)
+                sum += parts[k * stride + i];
+            out[i] = from_float<T>(sum);
+        }
+    }
+}
+
 // ------------------------------------------------------------ the epilogue's gradient
 // dz = grad act'(z), rounded once to the operands' type (for the two products
 // behind it: a second rounding of the size of their results'), and the bias

@@ -425,6 +425,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
                  : "memory");
 }
 
+// The same without a release: for an arrival that hands over tensor memory
+// only (ordered by tcgen05.fence), where a release would first wait for the
+// thread's outstanding global stores.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+                 : "memory");
+}
+
 // TMA load into this CTA's shared memory whose completion is counted on an
 // mbarrier of either CTA of the pair (2-CTA MMA pipelines).  No multicast.
 __device__ __forceinline__ void tma_load_5d_pair(void *dst, const CUtensorMap *map,

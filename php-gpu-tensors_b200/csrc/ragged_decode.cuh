@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     if (threadIdx.x == 0) {
         if (p.inner > 0) {
             prefetch_tensor_map(&maps.a);
-            prefetch_tensor_map(&maps.b16);
+            prefetch_tensor_map(&maps.rows[0]);
         }
         for (int s = 0; s < S; s++) {
             mbar_init(&full[s], 1);
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
     }
     const int rows = live ? min(kDecodeRows, n_end - n0) : 0;
     const int n = (rows + 15) & ~15;
+    const int box = row_box(n);
     const int blocks = (p.inner + 63) / 64;
     const int kb0 = static_cast<int>(static_cast<long long>(blocks) * rank / split);
     const int kb1 = live ? static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / split)
@@ -116,17 +117,18 @@ __global__ void __launch_bounds__(kDecodeThreads)
             }
             uint8_t *sa = smem + stage * kDecodeStage;
             uint8_t *sb = sa + kDecodeATile;
-            mbar_arrive_expect_tx(&full[stage], kDecodeATile + n * 128);
+            mbar_arrive_expect_tx(&full[stage], kDecodeATile + (2048 << box));
             const int k = kb * 64;
-            if (p.a_mn) {
+            if (!p.a_mn) {
+                tma_load_5d(sa, &maps.a, &full[stage], k, f0, group, 0, 0);
+            } else if (p.a_chunks) {
+                tma_load_5d(sa, &maps.a, &full[stage], 0, k, f0 >> 6, group, 0);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 2; j++)
                     tma_load_5d(sa + j * 8192, &maps.a, &full[stage], f0 + j * 64, k, group, 0, 0);
-            } else {
-                tma_load_5d(sa, &maps.a, &full[stage], k, f0, group, 0, 0);
             }
-            for (int j = 0; j < n / 16; j++)
-                tma_load_5d(sb + j * 2048, &maps.b16, &full[stage], k, n0 + j * 16, 0, 0, 0);
+            tma_load_5d(sb, &maps.rows[box], &full[stage], k, n0, 0, 0, 0);
             issued++;
             if (++stage == S) {
                 stage = 0;

@@ -46,40 +46,67 @@ struct RaggedParams {
     int cols;                 // INNER: N side
     int inner;                // COLS: K
     int a_mn;                 // COLS: the weight's features are contiguous
+    int a_chunks, b_chunks;   // that map walks 64-element chunks: one load per stage
     int passes;               // CHUNKED: products of parts per k-block, 3 or 6
+    int span;                 // rows (INNER: columns) of a tile: 256, 128 or 64
+    int split;                // INNER: parts of a group's rows, each with its own result
     int act;
     uint32_t idesc;           // instruction descriptor without its N field
     void *out, *pre;
     long long out_row, out_group;       // element strides of the result
+    long long out_part;                 // INNER: between the parts' results
     const void *bias;
     int bias_f32;
     const void *residual;
     long long residual_row, residual_inner;   // element strides
+    int residual_small;                 // its offsets fit 32 bits
+    int tma_store;                      // 16-bit results leave through maps.out and maps.pre
     const CUtensorMap *group_maps;      // INNER, several groups: a and b of each group
     int *status;
 };
 
+// A load costs the thread that issues it some 0.1 us on B200 (4096 of K: 0.35 us a
+// k-block with three loads, 0.43 with four), a third of a k-block's
+// MMAs at N = 256.  So a stage is two loads, by two threads: operands
+// that are contiguous along features (or INNER: columns) have a map
+// of dims (64, k, chunk of 64), whose one box is both of a CTA's chunks,
+// where the axis is a multiple of 64; rows come in the smallest of four
+// boxes that holds them.
 struct RaggedMaps {
     CUtensorMap a;            // features
-    CUtensorMap b;            // rows: a box of half a tile (COLS), or as a (INNER)
-    CUtensorMap b16;          // COLS: the same in boxes of 16 rows
+    CUtensorMap b;            // INNER: columns
+    CUtensorMap rows[4];      // COLS: boxes of 16, 32, 64 and 128 rows
+    CUtensorMap out, pre;     // results, in boxes of 32 features x kGroup rows
 };
 
 constexpr int kMaxGroups = 2048;
 constexpr int kRaggedBN = 256;
 constexpr int kRaggedStages = 6;
 // Sixteen epilogue warps hide each other's latencies (TMEM, residual, stores);
-// CHUNKED ones keep a tile's sums in registers, 64 each.
+// CHUNKED ones keep a tile's sums in registers, 64 each.  Warps 0 and the last
+// issue the loads of the two operands, warp 1 the MMAs.
 constexpr int kRaggedEpiWarps = 16;
-constexpr int kRaggedThreads = 32 * (2 + kRaggedEpiWarps);
+constexpr int kRaggedThreads = 32 * (3 + kRaggedEpiWarps);
+constexpr int kRaggedRowWarp = 2 + kRaggedEpiWarps;
 constexpr int kRaggedTile = 16384;                       // 128 rows x 64 of K, 16 bits
 constexpr int kRaggedRing = kRaggedStages * 2 * kRaggedTile;
 constexpr int kRaggedBars = 2 * kRaggedStages + 4 + 1;
-constexpr int kRaggedTableOffset = kRaggedRing + kRaggedBars * 8 + 24;
+// the epilogue works on kGroup rows at a time: a warp's box of 32 features
+constexpr int kGroup = 16;
+constexpr int kRaggedBox = kGroup * 32 * 2;
+constexpr int kRaggedBoxOffset = kRaggedRing;
+constexpr int kRaggedBarOffset = kRaggedBoxOffset + 16 * kRaggedBox;
+constexpr int kRaggedTableOffset = kRaggedBarOffset + kRaggedBars * 8 + 24;
 constexpr int kRaggedSmem = kRaggedTableOffset + 2 * kMaxGroups * 4 + 1024;
 static_assert(kRaggedSmem <= 232448, "shared memory budget exceeded");
 constexpr int kChunkBlocks = 2;                          // k-blocks of 64 per chunk
 constexpr int kFeatureBand = 8;                          // feature tiles walked per row tile
+
+// Index in RaggedMaps::rows of the smallest box that holds n rows.
+__device__ __forceinline__ int row_box(int n)
+{
+    return n <= 16 ? 0 : n <= 32 ? 1 : n <= 64 ? 2 : 3;
+}
 
 // Row ranges and tile counts of the groups, in shared memory.
 struct GroupTable {
@@ -155,11 +182,11 @@ __device__ __forceinline__ int group_end(const GroupTable &g, int i)
 
 // One tile of work.
 struct RaggedTile {
-    int group;
+    int group, part;
     int f0;          // first feature
     int n0, n_end;   // first row (COLS) or column (INNER), and the one behind the last
     int n;           // instruction N: a multiple of 32
-    int k0, k_end;   // range of the inner axis
+    int k0;          // start of its range of the inner axis
     int k_blocks;
 };
 
@@ -168,7 +195,7 @@ __device__ __forceinline__ long long ragged_tiles(const RaggedParams &p, const G
 {
     const long long ft = (p.features + 255) / 256;
     if (INNER)
-        return ft * ((p.cols + kRaggedBN - 1) / kRaggedBN) * p.groups;
+        return ft * ((p.cols + p.span - 1) / p.span) * p.groups * p.split;
     return ft * g.tiles[p.groups - 1];
 }
 
@@ -180,10 +207,12 @@ __device__ __forceinline__ RaggedTile ragged_tile(const RaggedParams &p, const G
     const int ft = (p.features + 255) / 256;
     int rows_t, local;
     if (INNER) {
-        rows_t = (p.cols + kRaggedBN - 1) / kRaggedBN;
+        rows_t = (p.cols + p.span - 1) / p.span;
         const int per = ft * rows_t;
-        r.group = static_cast<int>(t / per);
-        local = static_cast<int>(t - static_cast<long long>(r.group) * per);
+        const int unit = static_cast<int>(t / per);
+        local = static_cast<int>(t - static_cast<long long>(unit) * per);
+        r.group = unit / p.split;
+        r.part = unit - r.group * p.split;
     } else {
         r.group = find_group(g, static_cast<int>(t / ft));
         const int before = r.group > 0 ? g.tiles[r.group - 1] : 0;
@@ -199,18 +228,24 @@ __device__ __forceinline__ RaggedTile ragged_tile(const RaggedParams &p, const G
     r.f0 = (band * kFeatureBand + in_band % wide) * 256;
     const int start = g.start[r.group], end = group_end(g, r.group);
     if (INNER) {
-        r.n0 = nt * kRaggedBN;
+        // whole k-blocks for each part: only the group's last one may be ragged
+        const int blocks = (end - start + 63) / 64;
+        const int b0 = static_cast<int>(static_cast<long long>(blocks) * r.part / p.split);
+        const int b1 = static_cast<int>(static_cast<long long>(blocks) * (r.part + 1) / p.split);
+        r.n0 = nt * p.span;
         r.n_end = p.cols;
-        r.k0 = start;
-        r.k_end = end;
+        r.k0 = start + b0 * 64;
+        r.k_blocks = b1 - b0;
     } else {
-        r.n0 = start + nt * kRaggedBN;
+        r.part = 0;
+        r.n0 = start + nt * p.span;
         r.n_end = end;
         r.k0 = 0;
-        r.k_end = p.inner;
+        r.k_blocks = (p.inner + 63) / 64;
     }
-    r.n = min(kRaggedBN, (r.n_end - r.n0 + 31) & ~31);
-    r.k_blocks = (r.k_end - r.k0 + 63) / 64;
+    // (a map of chunks needs both CTAs' halves to be whole ones)
+    const int step = INNER && p.b_chunks ? 128 : 32;
+    r.n = min(p.span, (r.n_end - r.n0 + step - 1) & -step);
     return r;
 }
 
@@ -223,35 +258,72 @@ __device__ __forceinline__ void pass_parts(int passes, int q, int &pa, int &pb)
     pb = (0x046 >> shift) & 3;
 }
 
-// The epilogue works on kGroup rows at a time: lane = feature, so a warp
-// reads and writes 32 neighbouring features of each row.
-constexpr int kGroup = 16;
-
 // residual of rows n0 .. n0 + kGroup - 1 (those below count) at this feature.
+template <typename T, typename Offset>
+__device__ __forceinline__ void load_residual_at(const RaggedParams &p, int n0, int count,
+                                                 int feature, T (&r)[kGroup])
+{
+    const T *base = static_cast<const T *>(p.residual);
+    const Offset step = static_cast<Offset>(p.residual_row);
+    const Offset at = static_cast<Offset>(n0) * step +
+                      static_cast<Offset>(feature) * static_cast<Offset>(p.residual_inner);
+    if (count >= kGroup) {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            r[j] = __ldg(base + (at + j * step));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kGroup; j++)
+            if (j < count)
+                r[j] = __ldg(base + (at + j * step));
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void load_residual(const RaggedParams &p, int n0, int count,
                                               int feature, T (&r)[kGroup])
 {
     if (feature >= p.features)
         return;
-    const T *q = static_cast<const T *>(p.residual) + feature * p.residual_inner +
-                 n0 * p.residual_row;
-    if (count >= kGroup) {
-#pragma unroll
-        for (int j = 0; j < kGroup; j++)
-            r[j] = __ldg(q + j * p.residual_row);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kGroup; j++)
-            if (j < count)
-                r[j] = __ldg(q + j * p.residual_row);
-    }
+    if (p.residual_small)
+        load_residual_at<T, uint32_t>(p, n0, count, feature, r);
+    else
+        load_residual_at<T, long long>(p, n0, count, feature, r);
 }
 
+// A group's values to their place: 32 lanes write 32 neighbouring features of
+// each row, through the warp's box and one TMA store (16-bit results; a lane's
+// shared-memory stores have constant offsets, where global ones would cost
+// address arithmetic each), or directly for the last rows of a group.
 template <typename T>
-__device__ __forceinline__ void store_group(T *out, long long ld, int count,
-                                            const float (&v)[kGroup])
+__device__ __forceinline__ void store_group(const RaggedParams &p, T *out, const CUtensorMap *map,
+                                            uint8_t *box, int n0, int count, int f_warp,
+                                            int group, const float (&v)[kGroup])
 {
+    const int lane = threadIdx.x & 31;
+    if constexpr (sizeof(T) == 2) {
+        if (p.tma_store && count >= kGroup) {
+            if (lane == 0)
+                bulk_wait_group_read<0>();       // the box's last store has read it
+            __syncwarp();
+            T *mine = reinterpret_cast<T *>(box) + lane;
+#pragma unroll
+            for (int j = 0; j < kGroup; j++)
+                mine[j * 32] = from_float<T>(v[j]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && f_warp < p.features) {
+                tma_store_5d(map, box, f_warp, n0, group, 0, 0);
+                bulk_commit_group();
+            }
+            return;
+        }
+    }
+    const int feature = f_warp + lane;
+    if (feature >= p.features)
+        return;
+    const long long ld = p.out_row;
+    out += n0 * ld + feature;
     if (count >= kGroup) {
 #pragma unroll
         for (int j = 0; j < kGroup; j++)
@@ -265,22 +337,23 @@ __device__ __forceinline__ void store_group(T *out, long long ld, int count,
 }
 
 // Bias, activation and residual (r, already loaded) on the values v of rows
-// n0 .. and their stores.
+// n0 .. and their stores.  Called by whole warps.
 template <typename T, bool INNER>
-__device__ __forceinline__ void finish_group(const RaggedParams &p, float (&v)[kGroup], int n0,
-                                             int count, int feature, float bias,
-                                             const T (&r)[kGroup], T *out, T *pre)
+__device__ __forceinline__ void finish_group(const RaggedParams &p, const RaggedMaps &maps,
+                                             float (&v)[kGroup], int n0, int count, int f_warp,
+                                             int group, float bias, const T (&r)[kGroup], T *out,
+                                             T *pre, uint8_t *box)
 {
     constexpr bool kFast = sizeof(T) == 2;
-    if (feature >= p.features || count <= 0)
+    if (count <= 0)
         return;
-    const long long ld = p.out_row;
     if constexpr (!INNER) {
+        const Float2 b2 = pair(bias, bias);
 #pragma unroll
-        for (int j = 0; j < kGroup; j++)
-            v[j] += bias;
+        for (int j = 0; j < kGroup; j += 2)
+            split(add2(pair(v[j], v[j + 1]), b2), v[j], v[j + 1]);
         if (pre)
-            store_group(pre + n0 * ld + feature, ld, count, v);
+            store_group(p, pre, &maps.pre, box, n0, count, f_warp, 0, v);
         if (p.act != CUDA_MATMUL_EPILOGUE_NONE)
             with_activation(p.act, [&](auto act) {
 #pragma unroll
@@ -293,7 +366,7 @@ __device__ __forceinline__ void finish_group(const RaggedParams &p, float (&v)[k
                 v[j] += to_float(r[j]);
         }
     }
-    store_group(out + n0 * ld + feature, ld, count, v);
+    store_group(p, out, &maps.out, box, n0, count, f_warp, INNER ? group : 0, v);
 }
 
 template <typename T>
@@ -354,7 +427,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kRaggedRing);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kRaggedBarOffset);
     uint64_t *full = bars;
     uint64_t *empty = bars + S;
     uint64_t *tfull = bars + 2 * S;
@@ -374,7 +447,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     if (warp == 0 && lane == 0) {
         if (INNER || p.inner > 0) {
             prefetch_tensor_map(&maps.a);
-            prefetch_tensor_map(&maps.b);
+            prefetch_tensor_map(INNER ? &maps.b : &maps.rows[3]);
         }
         for (int s = 0; s < S; s++) {
             mbar_init(&full[s], 1);
@@ -399,33 +472,35 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     grid_dependency_wait();
     grid_launch_dependents();
-    fill_groups(p.ends, p.groups, p.rows, kRaggedBN, table, table + kMaxGroups, total_end);
+    fill_groups(p.ends, p.groups, p.rows, p.span, table, table + kMaxGroups, total_end);
     const GroupTable groups = {table, table + kMaxGroups, p.groups, *total_end};
     const long long tiles = ragged_tiles<INNER>(p, groups);
     const int passes = CHUNKED ? p.passes : 1;
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ producer (both CTAs)
+    if (warp == 0 || warp == kRaggedRowWarp) {
+        // ------------------------------------------------------------ producers (both CTAs)
+        // warp 0: the features' operand, and the barrier's expected bytes; the
+        // last warp: the rows' operand
+        const bool first = warp == 0;
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
             uint32_t issued_mask = 0, parity_mask = 0;
             bool ok = true;
+            const uint32_t full_leader = map_to_cta(smem_addr(full), 0);
             for (long long t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const int half = r.n / 2;
                 const int f = r.f0 + static_cast<int>(rank) * 128;
                 const int n = r.n0 + static_cast<int>(rank) * half;
-                const int b_boxes = INNER ? (half + 63) / 64 : half == 128 ? 1 : half / 16;
-                const uint32_t bytes =
-                    kRaggedTile + (INNER ? b_boxes * 8192u : static_cast<uint32_t>(half) * 128u);
+                const int box = INNER ? 0 : row_box(half);
+                const int b_boxes = p.b_chunks ? 2 : (half + 63) / 64;
+                const uint32_t bytes = kRaggedTile + (INNER ? b_boxes * 8192u : 2048u << box);
                 const int iters = r.k_blocks * passes;
-                const CUtensorMap *map_a = &maps.a, *map_b = &maps.b;
+                const CUtensorMap *map = first ? &maps.a : INNER ? &maps.b : &maps.rows[box];
                 if (INNER && p.group_maps) {
-                    map_a = p.group_maps + 2 * r.group;
-                    map_b = map_a + 1;
-                    tensor_map_acquire(map_a);
-                    tensor_map_acquire(map_b);
+                    map = p.group_maps + 2 * r.group + (first ? 0 : 1);
+                    tensor_map_acquire(map);
                 }
                 for (int i = 0; i < iters; i++) {
                     int pa = 0, pb = 0, kb = i;
@@ -438,34 +513,30 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                         ok = false;
                         break;
                     }
-                    uint8_t *sa = smem + stage * 2 * kRaggedTile;
-                    uint8_t *sb = sa + kRaggedTile;
-                    if (rank == 0)
+                    uint8_t *to = smem + stage * 2 * kRaggedTile + (first ? 0 : kRaggedTile);
+                    if (first && rank == 0)
                         mbar_arrive_expect_tx(&full[stage], 2 * bytes);
-                    const uint32_t full0 = map_to_cta(smem_addr(&full[stage]), 0);
+                    const uint32_t full0 = full_leader + stage * 8;
                     const int k = r.k0 + kb * 64;
-                    if (INNER) {
-#pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            tma_load_5d_pair(sa + j * 8192, map_a, full0, f + j * 64, k, pa, 0, 0);
-                        for (int j = 0; j < b_boxes; j++)
-                            tma_load_5d_pair(sb + j * 8192, map_b, full0, n + j * 64, k, pb, 0, 0);
-                    } else {
-                        if (p.a_mn) {
+                    if (first) {
+                        if (!INNER && !p.a_mn) {
+                            tma_load_5d_pair(to, map, full0, k, f, r.group, pa, 0);
+                        } else if (p.a_chunks) {
+                            tma_load_5d_pair(to, map, full0, 0, k, f >> 6, INNER ? pa : r.group,
+                                             INNER ? 0 : pa);
+                        } else {
 #pragma unroll
                             for (int j = 0; j < 2; j++)
-                                tma_load_5d_pair(sa + j * 8192, &maps.a, full0, f + j * 64, k,
-                                                 r.group, pa, 0);
-                        } else {
-                            tma_load_5d_pair(sa, &maps.a, full0, k, f, r.group, pa, 0);
+                                tma_load_5d_pair(to + j * 8192, map, full0, f + j * 64, k,
+                                                 INNER ? pa : r.group, INNER ? 0 : pa, 0);
                         }
-                        if (half == 128) {
-                            tma_load_5d_pair(sb, &maps.b, full0, k, n, pb, 0, 0);
-                        } else {
-                            for (int j = 0; j < b_boxes; j++)
-                                tma_load_5d_pair(sb + j * 2048, &maps.b16, full0, k, n + j * 16,
-                                                 pb, 0, 0);
-                        }
+                    } else if (!INNER) {
+                        tma_load_5d_pair(to, map, full0, k, n, pb, 0, 0);
+                    } else if (p.b_chunks) {
+                        tma_load_5d_pair(to, map, full0, 0, k, n >> 6, pb, 0);
+                    } else {
+                        for (int j = 0; j < b_boxes; j++)
+                            tma_load_5d_pair(to + j * 8192, map, full0, n + j * 64, k, pb, 0, 0);
                     }
                     issued_mask |= 1u << stage;
                     parity_mask = (parity_mask & ~(1u << stage)) | (phase << stage);
@@ -475,7 +546,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     }
                 }
             }
-            if (rank == 0) {
+            if (first && rank == 0) {
                 // CTA 0's full barriers count both CTAs' bytes of every stage
                 // it posted: let them land (bounded, ignores the abort flag)
                 for (int s = 0; s < S; s++) {
@@ -497,8 +568,13 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             bool ok = true;
             const uint32_t smem_base = smem_addr(smem);
             const bool a_mn = INNER || p.a_mn;
-            const uint32_t a_lbo = a_mn ? 8192 : 16, a_step = a_mn ? 16 * 128 : 32;
-            const uint32_t b_lbo = INNER ? 8192 : 16, b_step = INNER ? 16 * 128 : 32;
+            // descriptors of stage 0; a step of 16 bytes adds one to them
+            const uint64_t a0 = smem_desc(smem_base, a_mn ? 8192 : 16, 1024, kLayoutSw128);
+            const uint64_t b0 =
+                smem_desc(smem_base + kRaggedTile, INNER ? 8192 : 16, 1024, kLayoutSw128);
+            const uint32_t a_step = (a_mn ? 16 * 128 : 32) / 16;
+            constexpr uint32_t kBStep = (INNER ? 16 * 128 : 32) / 16;
+            const uint32_t empty0 = smem_addr(empty), empty1 = map_to_cta(empty0, 1);
             for (long long t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const uint32_t idesc = p.idesc | (static_cast<uint32_t>(r.n >> 3) << 17);
@@ -525,19 +601,14 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t sa = smem_base + stage * 2 * kRaggedTile;
-                        const uint32_t sb = sa + kRaggedTile;
+                        const uint64_t ad = a0 + stage * (2 * kRaggedTile / 16);
+                        const uint64_t bd = b0 + stage * (2 * kRaggedTile / 16);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint64_t ad =
-                                smem_desc(sa + k * a_step, a_lbo, 1024, kLayoutSw128);
-                            const uint64_t bd =
-                                smem_desc(sb + k * b_step, b_lbo, 1024, kLayoutSw128);
-                            umma_f16_pair(d_tmem, ad, bd, idesc, (i | k) != 0);
-                        }
-                        const uint32_t e0 = smem_addr(&empty[stage]);
-                        umma_commit_pair(e0);
-                        umma_commit_pair(map_to_cta(e0, 1));
+                        for (int k = 0; k < 4; k++)
+                            umma_f16_pair(d_tmem, ad + k * a_step, bd + k * kBStep, idesc,
+                                          (i | k) != 0);
+                        umma_commit_pair(empty0 + stage * 8);
+                        umma_commit_pair(empty1 + stage * 8);
                         if (++stage == S) {
                             stage = 0;
                             phase ^= 1;
@@ -558,15 +629,18 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
         // ------------------------------------------------------------ epilogue (both CTAs)
         const int quad = warp & 3;                     // TMEM lane quadrant of this warp
         const int side = (warp - 2) >> 2;              // its kCols of the 256 columns
+        uint8_t *box = smem + kRaggedBoxOffset + (warp - 2) * kRaggedBox;
         constexpr int kCols = kRaggedBN / (kEpiWarps / 4);
         long long chunk = 0;
         bool ok = true;
         for (long long t = cluster; ok && t < tiles; t += nclusters) {
             const RaggedTile r = ragged_tile<INNER>(p, groups, t);
-            const int feature = r.f0 + static_cast<int>(rank) * 128 + quad * 32 + lane;
-            const int mine = min(max(r.n - side * kCols, 0), kCols);   // multiple of 32
+            const int f_warp = r.f0 + static_cast<int>(rank) * 128 + quad * 32;
+            const int feature = f_warp + lane;
+            const int mine = min(max(r.n - side * kCols, 0), kCols);
             const int n0 = r.n0 + side * kCols;
-            T *out = static_cast<T *>(p.out) + (INNER ? r.group * p.out_group : 0);
+            T *out = static_cast<T *>(p.out) +
+                     (INNER ? r.group * p.out_group + r.part * p.out_part : 0);
             T *pre = static_cast<T *>(p.pre);
             float bias = 0.0f;
             T res[kGroup];
@@ -635,8 +709,13 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                         tmem_ld_wait_regs(raw);
 #pragma unroll
                         for (int j = 0; j < kGroup; j++) {
-                            v[j] = r.k_blocks > 0 ? __uint_as_float(raw[j]) : 0.0f;
+                            v[j] = __uint_as_float(raw[j]);
                             now[j] = res[j];
+                        }
+                        if (r.k_blocks == 0) {       // a sum over nothing
+#pragma unroll
+                            for (int j = 0; j < kGroup; j++)
+                                v[j] = 0.0f;
                         }
                         if (h + kGroup < mine) {
                             tmem_ld_32x32b_x16(t_acc + h + kGroup, raw);
@@ -646,17 +725,20 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                                                   feature, res);
                             }
                         }
-                        finish_group<T, INNER>(p, v, n0 + h, r.n_end - (n0 + h), feature, bias, now,
-                                               out, pre);
+                        finish_group<T, INNER>(p, maps, v, n0 + h, r.n_end - (n0 + h), f_warp,
+                                               r.group, bias, now, out, pre, box);
                         __syncwarp();
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive_cluster(map_to_cta(smem_addr(&tempty[acc]), 0));
+                    mbar_arrive_cluster_relaxed(map_to_cta(smem_addr(&tempty[acc]), 0));
             }
         }
+        if (lane == 0)
+            bulk_wait_group<0>();
+        __syncwarp();
         if (!INNER && groups.end < p.rows)
             zero_ungrouped<T>(p, groups.end, blockIdx.x * kEpiWarps + warp - 2,
                               gridDim.x * kEpiWarps);

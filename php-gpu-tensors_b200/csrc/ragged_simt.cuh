@@ -32,7 +32,7 @@ constexpr int kSimtThreads = 256;
 template <int TF, int TR>
 constexpr int ragged_simt_smem(int groups)
 {
-    return (2 * kSimtStep * (TF + TR + 4) + TF * TR) * 4 + 8 * groups;
+    return (2 * kSimtStep * (TF + TR + 8) + TF * TR) * 4 + 8 * groups;
 }
 
 template <typename T, bool INNER, int TF, int TR>
@@ -40,11 +40,13 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
 {
     constexpr int NR = TF * TR / (4 * kSimtThreads);
     constexpr int LB = kSimtStep * TF / kSimtThreads, LA = kSimtStep * TR / kSimtThreads;
-    constexpr int AP = TR + 4;
-    static_assert(NR >= 1 && LA >= 1, "tile too small for the block");
+    // pitches: four more floats keep 16-byte reads aligned and spread a column's
+    // writes over eight banks
+    constexpr int AP = TR + 4, BP = TF + 4;
+    static_assert(NR >= 2 && NR % 2 == 0 && LA >= 1, "tile too small for the block");
     extern __shared__ float simt_smem[];
-    float *bs = simt_smem;                               // [2][kSimtStep][TF]
-    float *as = bs + 2 * kSimtStep * TF;                 // [2][kSimtStep][AP]
+    float *bs = simt_smem;                               // [2][kSimtStep][BP]
+    float *as = bs + 2 * kSimtStep * BP;                 // [2][kSimtStep][AP]
     float *partial = as + 2 * kSimtStep * AP;            // [TR][TF]
     int *table = reinterpret_cast<int *>(partial + TF * TR);
     __shared__ int total_end;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
             const int e = j * kSimtThreads + tid;
             const int i = b_by_col ? e / TF : e % kSimtStep;
             const int f = b_by_col ? e % TF : e / kSimtStep;
-            bs[(buf * kSimtStep + i) * TF + f] = rb[j];
+            bs[(buf * kSimtStep + i) * BP + f] = rb[j];
         }
 #pragma unroll
         for (int j = 0; j < LA; j++) {
@@ -129,7 +131,10 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
     };
 
     const int tx = tid % (TF / 4), ty = tid / (TF / 4);
-    float acc[NR][4] = {};
+    Float2 acc[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+        acc[r][0] = acc[r][1] = pair(0.0f, 0.0f);
     if (s0 < s1)
         fetch(s0);
     for (int step = s0; step < s1; step++) {
@@ -141,21 +146,34 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
 #pragma unroll 8
         for (int i = 0; i < kSimtStep; i++) {
             const float4 q = *reinterpret_cast<const float4 *>(
-                &bs[(buf * kSimtStep + i) * TF + tx * 4]);
+                &bs[(buf * kSimtStep + i) * BP + tx * 4]);
+            const Float2 q0 = pair(q.x, q.y), q1 = pair(q.z, q.w);
+            float x[NR];
+            const float *xs = &as[(buf * kSimtStep + i) * AP + ty * NR];
+            if constexpr (NR % 4 == 0) {
+#pragma unroll
+                for (int r = 0; r < NR; r += 4)
+                    *reinterpret_cast<float4 *>(x + r) = *reinterpret_cast<const float4 *>(xs + r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; r += 2)
+                    *reinterpret_cast<float2 *>(x + r) = *reinterpret_cast<const float2 *>(xs + r);
+            }
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const float x = as[(buf * kSimtStep + i) * AP + ty * NR + r];
-                acc[r][0] = fmaf(x, q.x, acc[r][0]);
-                acc[r][1] = fmaf(x, q.y, acc[r][1]);
-                acc[r][2] = fmaf(x, q.z, acc[r][2]);
-                acc[r][3] = fmaf(x, q.w, acc[r][3]);
+                const Float2 xx = pair(x[r], x[r]);
+                acc[r][0] = fma2(xx, q0, acc[r][0]);
+                acc[r][1] = fma2(xx, q1, acc[r][1]);
             }
         }
     }
 #pragma unroll
-    for (int r = 0; r < NR; r++)
-        *reinterpret_cast<float4 *>(&partial[(ty * NR + r) * TF + tx * 4]) =
-            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    for (int r = 0; r < NR; r++) {
+        float4 q;
+        split(acc[r][0], q.x, q.y);
+        split(acc[r][1], q.z, q.w);
+        *reinterpret_cast<float4 *>(&partial[(ty * NR + r) * TF + tx * 4]) = q;
+    }
     if (s.split > 1)
         cluster_sync();
     else

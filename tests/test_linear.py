@@ -144,7 +144,7 @@ def check_backward(c, out, dtype, act, spans, dw_dtype=None):
 
 
 # a case beyond one tile of each kernel in every direction, and odd ones
-SIZES = [(1, 64, 64), (65, 2100, 130), (2, 8, 8), (3, 7, 5), (8, 128, 264), (31, 65, 1), (33, 1, 70), (129, 72, 520),
+SIZES = [(1, 64, 64), (65, 2100, 130), (2100, 130, 72), (2, 8, 8), (3, 7, 5), (8, 128, 264), (31, 65, 1), (33, 1, 70), (129, 72, 520),
          (256, 256, 256), (257, 200, 96), (300, 1000, 136), (700, 264, 312)]
 
 
@@ -205,7 +205,7 @@ def test_layouts(dtype, layout, path):
     check_forward(c, y.to_torch(), None, dtype, "silu", [(0, 150)])
 
 
-ENDS = [[0, 0, 5, 5, 40], [64, 128, 192, 256], [1, 2, 3, 400], [300], [0, 0, 0],
+ENDS = [[0, 0, 5, 5, 40], [1800, 1800, 1843], [64, 128, 192, 256], [1, 2, 3, 400], [300], [0, 0, 0],
         [255, 256, 513, 514, 600], [10, 4, 90, 70, 5000]]      # the last one: not in order
 
 
