@@ -547,4 +547,15 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_addr)
                  : "memory");
 }
 
+// umma_commit_pair to the barrier at this shared-memory offset in both CTAs of
+// the pair (cluster ranks 0 and 1), as one operation.
+__device__ __forceinline__ void umma_commit_pair_both(uint32_t smem_addr_local)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_addr_local),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
 } // namespace ptg

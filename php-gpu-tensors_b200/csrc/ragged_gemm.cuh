@@ -14,7 +14,7 @@
 //
 // A cluster of two CTAs computes 256 features x up to 256 rows: CTA r loads
 // features [128 r, 128 r + 128) and half of the rows, 64 of K at a time, into
-// a 6-stage ring of 128-byte-swizzled tiles.  Warp 0 issues the TMA loads,
+// a ring of 128-byte-swizzled tiles.  Warp 0 issues the TMA loads,
 // warp 1 of CTA 0 the MMAs into one of two 256-column accumulators, the other
 // warps read the other one, apply bias, activation and residual and store.
 // Barriers as in gemm_tc2.cuh; every wait is bounded.  No TMA multicast.
@@ -81,7 +81,11 @@ struct RaggedMaps {
 
 constexpr int kMaxGroups = 2048;
 constexpr int kRaggedBN = 256;
-constexpr int kRaggedStages = 6;
+// A stage is two k-blocks: waits and commits hold up the thread that issues the
+// MMAs (8192^3 bfloat16: a commit to each CTA per k-block 776 us, one to both
+// 751), so there is one of each for eight MMAs.
+constexpr int kRaggedStages = 3;
+constexpr int kStageKb = 2;
 // Sixteen epilogue warps hide each other's latencies (TMEM, residual, stores);
 // CHUNKED ones keep a tile's sums in registers, 64 each.  Warps 0 and the last
 // issue the loads of the two operands, warp 1 the MMAs.
@@ -89,7 +93,9 @@ constexpr int kRaggedEpiWarps = 16;
 constexpr int kRaggedThreads = 32 * (3 + kRaggedEpiWarps);
 constexpr int kRaggedRowWarp = 2 + kRaggedEpiWarps;
 constexpr int kRaggedTile = 16384;                       // 128 rows x 64 of K, 16 bits
-constexpr int kRaggedRing = kRaggedStages * 2 * kRaggedTile;
+constexpr int kRaggedKb = 2 * kRaggedTile;               // both operands of a k-block
+constexpr int kRaggedStage = kStageKb * kRaggedKb;
+constexpr int kRaggedRing = kRaggedStages * kRaggedStage;
 constexpr int kRaggedBars = 2 * kRaggedStages + 4 + 1;
 // the epilogue works on kGroup rows at a time: a warp's box of 32 features
 constexpr int kGroup = 16;
@@ -100,6 +106,7 @@ constexpr int kRaggedTableOffset = kRaggedBarOffset + kRaggedBars * 8 + 24;
 constexpr int kRaggedSmem = kRaggedTableOffset + 2 * kMaxGroups * 4 + 1024;
 static_assert(kRaggedSmem <= 232448, "shared memory budget exceeded");
 constexpr int kChunkBlocks = 2;                          // k-blocks of 64 per chunk
+static_assert(kChunkBlocks % kStageKb == 0, "stages do not straddle chunks");
 constexpr int kFeatureBand = 8;                          // feature tiles walked per row tile
 
 // Index in RaggedMaps::rows of the smallest box that holds n rows.
@@ -502,41 +509,49 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     map = p.group_maps + 2 * r.group + (first ? 0 : 1);
                     tensor_map_acquire(map);
                 }
-                for (int i = 0; i < iters; i++) {
-                    int pa = 0, pb = 0, kb = i;
-                    if (CHUNKED) {
-                        kb = i / passes;
-                        pass_parts(passes, i - kb * passes, pa, pb);
-                    }
+                for (int i = 0; i < iters; i += kStageKb) {
+                    const int count = min(kStageKb, iters - i);
                     if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
                         record_failure(abort, p.status, DEV_TIMEOUT_PRODUCER);
                         ok = false;
                         break;
                     }
-                    uint8_t *to = smem + stage * 2 * kRaggedTile + (first ? 0 : kRaggedTile);
                     if (first && rank == 0)
-                        mbar_arrive_expect_tx(&full[stage], 2 * bytes);
+                        mbar_arrive_expect_tx(&full[stage], count * 2 * bytes);
                     const uint32_t full0 = full_leader + stage * 8;
-                    const int k = r.k0 + kb * 64;
-                    if (first) {
-                        if (!INNER && !p.a_mn) {
-                            tma_load_5d_pair(to, map, full0, k, f, r.group, pa, 0);
-                        } else if (p.a_chunks) {
-                            tma_load_5d_pair(to, map, full0, 0, k, f >> 6, INNER ? pa : r.group,
-                                             INNER ? 0 : pa);
-                        } else {
 #pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                tma_load_5d_pair(to + j * 8192, map, full0, f + j * 64, k,
-                                                 INNER ? pa : r.group, INNER ? 0 : pa, 0);
+                    for (int sub = 0; sub < kStageKb; sub++) {
+                        if (sub >= count)
+                            break;
+                        int pa = 0, pb = 0, kb = i + sub;
+                        if (CHUNKED) {
+                            kb = (i + sub) / passes;
+                            pass_parts(passes, i + sub - kb * passes, pa, pb);
                         }
-                    } else if (!INNER) {
-                        tma_load_5d_pair(to, map, full0, k, n, pb, 0, 0);
-                    } else if (p.b_chunks) {
-                        tma_load_5d_pair(to, map, full0, 0, k, n >> 6, pb, 0);
-                    } else {
-                        for (int j = 0; j < b_boxes; j++)
-                            tma_load_5d_pair(to + j * 8192, map, full0, n + j * 64, k, pb, 0, 0);
+                        uint8_t *to = smem + stage * kRaggedStage + sub * kRaggedKb +
+                                      (first ? 0 : kRaggedTile);
+                        const int k = r.k0 + kb * 64;
+                        if (first) {
+                            if (!INNER && !p.a_mn) {
+                                tma_load_5d_pair(to, map, full0, k, f, r.group, pa, 0);
+                            } else if (p.a_chunks) {
+                                tma_load_5d_pair(to, map, full0, 0, k, f >> 6,
+                                                 INNER ? pa : r.group, INNER ? 0 : pa);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 2; j++)
+                                    tma_load_5d_pair(to + j * 8192, map, full0, f + j * 64, k,
+                                                     INNER ? pa : r.group, INNER ? 0 : pa, 0);
+                            }
+                        } else if (!INNER) {
+                            tma_load_5d_pair(to, map, full0, k, n, pb, 0, 0);
+                        } else if (p.b_chunks) {
+                            tma_load_5d_pair(to, map, full0, 0, k, n >> 6, pb, 0);
+                        } else {
+                            for (int j = 0; j < b_boxes; j++)
+                                tma_load_5d_pair(to + j * 8192, map, full0, n + j * 64, k, pb, 0,
+                                                 0);
+                        }
                     }
                     issued_mask |= 1u << stage;
                     parity_mask = (parity_mask & ~(1u << stage)) | (phase << stage);
@@ -574,7 +589,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                 smem_desc(smem_base + kRaggedTile, INNER ? 8192 : 16, 1024, kLayoutSw128);
             const uint32_t a_step = (a_mn ? 16 * 128 : 32) / 16;
             constexpr uint32_t kBStep = (INNER ? 16 * 128 : 32) / 16;
-            const uint32_t empty0 = smem_addr(empty), empty1 = map_to_cta(empty0, 1);
+            const uint32_t empty0 = smem_addr(empty);
             for (long long t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const uint32_t idesc = p.idesc | (static_cast<uint32_t>(r.n >> 3) << 17);
@@ -594,21 +609,26 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kRaggedBN);
                     const int n = min(per, left);
                     left -= n;
-                    for (int i = 0; i < n; i++) {
+                    for (int i = 0; i < n; i += kStageKb) {
                         if (!mbar_wait(&full[stage], phase, abort)) {
                             record_failure(abort, p.status, DEV_TIMEOUT_MMA);
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t ad = a0 + stage * (2 * kRaggedTile / 16);
-                        const uint64_t bd = b0 + stage * (2 * kRaggedTile / 16);
+                        const uint64_t ad = a0 + stage * (kRaggedStage / 16);
+                        const uint64_t bd = b0 + stage * (kRaggedStage / 16);
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            umma_f16_pair(d_tmem, ad + k * a_step, bd + k * kBStep, idesc,
-                                          (i | k) != 0);
-                        umma_commit_pair(empty0 + stage * 8);
-                        umma_commit_pair(empty1 + stage * 8);
+                        for (int sub = 0; sub < kStageKb; sub++) {
+                            if (i + sub >= n)
+                                break;
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                umma_f16_pair(d_tmem, ad + sub * (kRaggedKb / 16) + k * a_step,
+                                              bd + sub * (kRaggedKb / 16) + k * kBStep, idesc,
+                                              (i | sub | k) != 0);
+                        }
+                        umma_commit_pair_both(empty0 + stage * 8);
                         if (++stage == S) {
                             stage = 0;
                             phase ^= 1;
@@ -616,9 +636,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     }
                     if (!ok)
                         break;
-                    const uint32_t f0 = smem_addr(&tfull[acc]);
-                    umma_commit_pair(f0);
-                    umma_commit_pair(map_to_cta(f0, 1));
+                    umma_commit_pair_both(smem_addr(&tfull[acc]));
                 } while (left > 0);
             }
             umma_commit_pair(smem_addr(drain));
