@@ -388,10 +388,10 @@ bool few_rows(const PtgDevice &dev, long long pair_tiles, int rows, int groups)
 // ------------------------------------------------------------ CUDA cores
 constexpr int kSimtFewRows = 16;
 
-template <typename T, bool INNER, int TF, int TR>
+template <typename T, typename TZ, bool INNER, int TF, int TR>
 cudaError_t launch_simt_tile(const Plan &pl, RaggedSimtParams &s)
 {
-    constexpr auto kernel = ragged_simt_kernel<T, INNER, TF, TR>;
+    constexpr auto kernel = ragged_simt_kernel<T, TZ, INNER, TF, TR>;
     static std::mutex mutex;
     static bool ready[kMaxDevices] = {};
     int device = 0;
@@ -437,18 +437,33 @@ cudaError_t launch_simt_tile(const Plan &pl, RaggedSimtParams &s)
     return cudaLaunchKernelEx(&cfg, kernel, s);
 }
 
-template <typename T, bool INNER>
-cudaError_t launch_simt(const Plan &pl, RaggedSimtParams &s)
+template <typename T, typename TZ, bool INNER>
+cudaError_t launch_simt_rows(const Plan &pl, RaggedSimtParams &s)
 {
     const int rows = INNER ? s.p.cols : (s.p.rows + s.p.groups - 1) / s.p.groups;
-    return rows <= kSimtFewRows ? launch_simt_tile<T, INNER, 128, 16>(pl, s)
-                                : launch_simt_tile<T, INNER, 64, 64>(pl, s);
+    return rows <= kSimtFewRows ? launch_simt_tile<T, TZ, INNER, 128, 16>(pl, s)
+                                : launch_simt_tile<T, TZ, INNER, 64, 64>(pl, s);
+}
+
+template <bool INNER>
+cudaError_t launch_simt(const Plan &pl, RaggedSimtParams &s, int dtype, bool z_f32)
+{
+    switch (dtype) {
+    case DTYPE_FLOAT16:
+        return z_f32 ? launch_simt_rows<__half, float, INNER>(pl, s)
+                     : launch_simt_rows<__half, __half, INNER>(pl, s);
+    case DTYPE_BFLOAT16:
+        return z_f32 ? launch_simt_rows<__nv_bfloat16, float, INNER>(pl, s)
+                     : launch_simt_rows<__nv_bfloat16, __nv_bfloat16, INNER>(pl, s);
+    default: return launch_simt_rows<float, float, INNER>(pl, s);
+    }
 }
 
 // A matrix of rows with one stride each, in the operands' own type.
 struct Plain {
     const void *p;
     long long row, inner;
+    bool f32;           // float32 whatever the operands' type (a gradient's dz)
 };
 
 // Rows x weight as product() does it.
@@ -472,11 +487,7 @@ cudaError_t simt_product(Plan &pl, const PtgLinear &a, const Plain &x, bool tran
     s.b_inner = transposed ? a.w_cols : a.w_inner;
     s.b_col = transposed ? a.w_inner : a.w_cols;
     s.b_group = a.w_group;
-    switch (a.dtype) {
-    case DTYPE_FLOAT16: return launch_simt<__half, false>(pl, s);
-    case DTYPE_BFLOAT16: return launch_simt<__nv_bfloat16, false>(pl, s);
-    default: return launch_simt<float, false>(pl, s);
-    }
+    return launch_simt<false>(pl, s, a.dtype, x.f32);
 }
 
 // dw as weight_product() does it; the result has the operands' type.
@@ -500,11 +511,7 @@ cudaError_t simt_weight_product(Plan &pl, const PtgLinear &a, const Plain &x,
     s.b = dz.p;
     s.b_inner = dz.row;
     s.b_col = dz.inner;
-    switch (a.dtype) {
-    case DTYPE_FLOAT16: return launch_simt<__half, true>(pl, s);
-    case DTYPE_BFLOAT16: return launch_simt<__nv_bfloat16, true>(pl, s);
-    default: return launch_simt<float, true>(pl, s);
-    }
+    return launch_simt<true>(pl, s, a.dtype, dz.f32);
 }
 
 // A view's own rows, or a contiguous copy where they have no single stride.
@@ -512,7 +519,7 @@ Plain plan_plain(Plan &pl, int dtype, const void *src, const RowView &v, long lo
                  long long rows, int cols)
 {
     if (v.n == 1)
-        return {src, v.stride[0], inner};
+        return {src, v.stride[0], inner, false};
     void *out = pl.ws.take(static_cast<size_t>(rows) * cols * element_bytes(dtype));
     if (pl.run && pl.ok()) {
         const long long blocks = (rows * cols + 255) / 256;
@@ -526,7 +533,7 @@ Plain plan_plain(Plan &pl, int dtype, const void *src, const RowView &v, long lo
                            static_cast<const uint16_t *>(src), v, inner, rows, cols,
                            static_cast<uint16_t *>(out)));
     }
-    return {out, cols, 1};
+    return {out, cols, 1, false};
 }
 
 // ------------------------------------------------------------ tensor cores
@@ -721,6 +728,7 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
 // 1 and 3: the tensor-core kernels).
 constexpr double kSimtWork = 5.0e8;
 constexpr double kSimtLayWork = 5.0e7;
+constexpr double kExactGradient = 16384;
 
 bool on_cuda_cores(const PtgLinear &a, bool lay)
 {
@@ -820,7 +828,12 @@ void backward(Plan &pl, const PtgLinear &a)
     const bool products = a.dx || a.dw;
     const bool lay = (!active && needs_layout(a, a.grad, a.gv, a.g_inner, a.cols)) ||
                      needs_layout(a, a.x, a.xv, a.x_inner, a.inner);
-    const bool simt = on_cuda_cores(a, lay) && (!a.dw || a.dw_dtype == a.dtype);
+    // dz of a few rows stays in float32: below some thousand elements its
+    // roundings to 16 bits would not average out in the products
+    const bool exact = a.dtype != DTYPE_FLOAT32 && active &&
+                       static_cast<double>(a.rows) * a.cols <= kExactGradient;
+    const bool simt = (on_cuda_cores(a, lay) || (exact && ptg_path() == 0)) &&
+                      (!a.dw || a.dw_dtype == a.dtype);
     const size_t partial_rows = a.rows / kSlopeRows + std::min(a.groups, a.rows);
     float *partial = a.dbias ? static_cast<float *>(pl.ws.take(partial_rows * a.cols * 4)) : nullptr;
 
@@ -834,10 +847,10 @@ void backward(Plan &pl, const PtgLinear &a)
     if (products && (active || (a.dtype == DTYPE_FLOAT32 && !simt))) {
         dz.ld = round8(a.cols);
         dz.part = a.rows * dz.ld;
-        const size_t each = a.dtype == DTYPE_FLOAT32 && simt ? 4 : 2 * static_cast<size_t>(pl.parts);
+        const size_t each = simt ? 4 : 2 * static_cast<size_t>(pl.parts);
         void *out = pl.ws.take(static_cast<size_t>(dz.part) * each);
         dz.p = out;
-        plain = {out, dz.ld, 1};
+        plain = {out, dz.ld, 1, true};
         if (pl.run && pl.ok())
             slope(pl, a, out, simt ? 0 : pl.parts, partial);
     } else {

@@ -156,6 +156,16 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, int 
 constexpr int kSlopeRows = 64;
 constexpr int kSlopeCols = 256;
 
+// Eight values as 16 bytes of a 16-bit type (unused for float).
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&v)[8])
+{
+    if constexpr (sizeof(T) == 2)
+        return pack_vec<T, 16>(v);
+    else
+        return uint4{};
+}
+
 struct SlopeParams {
     const void *grad, *pre;
     RowView gv, pv;
@@ -167,7 +177,7 @@ struct SlopeParams {
     void *dz;               // [rows][ld]; null when grad itself serves
     int ld;
     long long part;         // float32: parts as in lay_out_kernel
-    int parts;
+    int parts;              // 0: dz stays in float32
     float *partial;         // [row tiles][cols], or null
     int strips;             // column strips: block = row tile * strips + strip
 };
@@ -218,8 +228,8 @@ __device__ __forceinline__ void slope_rows(const SlopeParams &p, int r0, int r1,
             if (p.dz) {
                 uint16_t *out =
                     static_cast<uint16_t *>(p.dz) + static_cast<long long>(r) * p.ld + c;
-                if constexpr (sizeof(T) == 2)
-                    *reinterpret_cast<uint4 *>(out) = pack_vec<T, 16>(v);
+                if (sizeof(T) == 2 && p.parts)
+                    *reinterpret_cast<uint4 *>(out) = pack16<T>(v);
                 else if (p.parts)
                     store_parts(v, out, p.part, p.parts);
                 else {

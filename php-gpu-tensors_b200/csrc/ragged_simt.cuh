@@ -6,7 +6,9 @@
 //
 // It serves float32 products that are too small for the split into bfloat16
 // parts to pay (its passes over the operands cost more than the products),
-// and 16-bit operands that would have to be laid out first.  For few rows
+// 16-bit operands that would have to be laid out first, and the gradients of
+// a few rows, whose dz stays in float32 (TZ): so few roundings to 16 bits
+// would not average out in the products.  For few rows
 // the weight's bytes bound it, else the multiply-adds.  A block makes a tile of TF
 // features x TR rows, four features x NR rows a thread, 32 of the inner axis
 // at a time through double-buffered shared memory, the next step's loads in
@@ -35,7 +37,7 @@ constexpr int ragged_simt_smem(int groups)
     return (2 * kSimtStep * (TF + TR + 8) + TF * TR) * 4 + 8 * groups;
 }
 
-template <typename T, bool INNER, int TF, int TR>
+template <typename T, typename TZ, bool INNER, int TF, int TR>
 __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedSimtParams s)
 {
     constexpr int NR = TF * TR / (4 * kSimtThreads);
@@ -43,6 +45,8 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
     // pitches: four more floats keep 16-byte reads aligned and spread a column's
     // writes over eight banks
     constexpr int AP = TR + 4, BP = TF + 4;
+    using TA = std::conditional_t<INNER, T, TZ>;
+    using TB = std::conditional_t<INNER, TZ, T>;
     static_assert(NR >= 2 && NR % 2 == 0 && LA >= 1, "tile too small for the block");
     extern __shared__ float simt_smem[];
     float *bs = simt_smem;                               // [2][kSimtStep][BP]
@@ -86,48 +90,53 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
     const int steps = live ? (k_end - k0 + kSimtStep - 1) / kSimtStep : 0;
     const int s0 = static_cast<int>(static_cast<long long>(steps) * rank / s.split);
     const int s1 = static_cast<int>(static_cast<long long>(steps) * (rank + 1) / s.split);
-    const T *a = static_cast<const T *>(s.a);
-    const T *b = static_cast<const T *>(s.b) + (INNER ? 0 : group * s.b_group);
+    const TA *a = static_cast<const TA *>(s.a);
+    const TB *b = static_cast<const TB *>(s.b) + (INNER ? 0 : group * s.b_group);
 
-    const bool b_by_col = s.b_col == 1 || s.b_inner != 1;     // which axis neighbours share
+    // Neighbouring threads read along the axis that is contiguous; every load of
+    // a thread then differs from its first by a fixed step, and its place on
+    // the other axis by a fixed count.
+    const bool b_by_col = s.b_col == 1 || s.b_inner != 1;
     const bool a_by_inner = s.a_inner == 1 || s.a_row != 1;
-    float ra[LA], rb[LB];
-    auto fetch = [&](int step) {
-        const int k = k0 + step * kSimtStep;
+    const int bi = b_by_col ? tid / TF : tid % kSimtStep;
+    const int bf = b_by_col ? tid % TF : tid / kSimtStep;
+    const int bi_step = b_by_col ? kSimtThreads / TF : 0;
+    const int bf_step = b_by_col ? 0 : kSimtThreads / kSimtStep;
+    const int ai = a_by_inner ? tid % kSimtStep : tid / TR;
+    const int ar = a_by_inner ? tid / kSimtStep : tid % TR;
+    const int ai_step = a_by_inner ? 0 : kSimtThreads / TR;
+    const int ar_step = a_by_inner ? kSimtThreads / kSimtStep : 0;
+    const long long b_step = bi_step * s.b_inner + bf_step * s.b_col;
+    const long long a_step = ai_step * s.a_inner + ar_step * s.a_row;
+    const long long first = k0 + static_cast<long long>(s0) * kSimtStep;
+    const TB *b_at = b + (first + bi) * s.b_inner + (f0 + bf) * s.b_col;
+    const TA *a_at = a + (n0 + ar) * s.a_row + (first + ai) * s.a_inner;
+    float ra[2][LA], rb[2][LB];
+    // the next step's elements into register set `set`; steps come in order
+    auto fetch = [&](int set, int step) {
+        const int left = k_end - (k0 + step * kSimtStep);
 #pragma unroll
-        for (int j = 0; j < LB; j++) {
-            const int e = j * kSimtThreads + tid;
-            const int i = b_by_col ? e / TF : e % kSimtStep;
-            const int f = b_by_col ? e % TF : e / kSimtStep;
-            rb[j] = k + i < k_end && f0 + f < p.features
-                        ? to_float(b[(k + i) * s.b_inner + (f0 + f) * s.b_col])
-                        : 0.0f;
-        }
+        for (int j = 0; j < LB; j++)
+            rb[set][j] = bi + j * bi_step < left && f0 + bf + j * bf_step < p.features
+                             ? to_float(b_at[j * b_step])
+                             : 0.0f;
 #pragma unroll
-        for (int j = 0; j < LA; j++) {
-            const int e = j * kSimtThreads + tid;
-            const int i = a_by_inner ? e % kSimtStep : e / TR;
-            const int r = a_by_inner ? e / kSimtStep : e % TR;
-            ra[j] = k + i < k_end && n0 + r < n_end
-                        ? to_float(a[(n0 + r) * s.a_row + (k + i) * s.a_inner])
-                        : 0.0f;
-        }
+        for (int j = 0; j < LA; j++)
+            ra[set][j] = ai + j * ai_step < left && n0 + ar + j * ar_step < n_end
+                             ? to_float(a_at[j * a_step])
+                             : 0.0f;
+        b_at += kSimtStep * s.b_inner;
+        a_at += kSimtStep * s.a_inner;
     };
-    auto put = [&](int buf) {
+    const int b_put = bi * BP + bf, b_put_step = bi_step * BP + bf_step;
+    const int a_put = ai * AP + ar, a_put_step = ai_step * AP + ar_step;
+    auto put = [&](int set) {
 #pragma unroll
-        for (int j = 0; j < LB; j++) {
-            const int e = j * kSimtThreads + tid;
-            const int i = b_by_col ? e / TF : e % kSimtStep;
-            const int f = b_by_col ? e % TF : e / kSimtStep;
-            bs[(buf * kSimtStep + i) * BP + f] = rb[j];
-        }
+        for (int j = 0; j < LB; j++)
+            bs[set * kSimtStep * BP + b_put + j * b_put_step] = rb[set][j];
 #pragma unroll
-        for (int j = 0; j < LA; j++) {
-            const int e = j * kSimtThreads + tid;
-            const int i = a_by_inner ? e % kSimtStep : e / TR;
-            const int r = a_by_inner ? e / kSimtStep : e % TR;
-            as[(buf * kSimtStep + i) * AP + r] = ra[j];
-        }
+        for (int j = 0; j < LA; j++)
+            as[set * kSimtStep * AP + a_put + j * a_put_step] = ra[set][j];
     };
 
     const int tx = tid % (TF / 4), ty = tid / (TF / 4);
@@ -135,35 +144,43 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
 #pragma unroll
     for (int r = 0; r < NR; r++)
         acc[r][0] = acc[r][1] = pair(0.0f, 0.0f);
-    if (s0 < s1)
-        fetch(s0);
-    for (int step = s0; step < s1; step++) {
-        const int buf = (step - s0) & 1;
-        put(buf);
-        __syncthreads();
-        if (step + 1 < s1)
-            fetch(step + 1);
+#pragma unroll
+    for (int set = 0; set < 2; set++)
+        if (s0 + set < s1)
+            fetch(set, s0 + set);
+    for (int base = s0; base < s1; base += 2) {
+#pragma unroll
+        for (int set = 0; set < 2; set++) {
+            if (base + set >= s1)
+                break;
+            put(set);
+            __syncthreads();
+            if (base + set + 2 < s1)
+                fetch(set, base + set + 2);
 #pragma unroll 8
-        for (int i = 0; i < kSimtStep; i++) {
-            const float4 q = *reinterpret_cast<const float4 *>(
-                &bs[(buf * kSimtStep + i) * BP + tx * 4]);
-            const Float2 q0 = pair(q.x, q.y), q1 = pair(q.z, q.w);
-            float x[NR];
-            const float *xs = &as[(buf * kSimtStep + i) * AP + ty * NR];
-            if constexpr (NR % 4 == 0) {
+            for (int i = 0; i < kSimtStep; i++) {
+                const float4 q = *reinterpret_cast<const float4 *>(
+                    &bs[(set * kSimtStep + i) * BP + tx * 4]);
+                const Float2 q0 = pair(q.x, q.y), q1 = pair(q.z, q.w);
+                float x[NR];
+                const float *xs = &as[(set * kSimtStep + i) * AP + ty * NR];
+                if constexpr (NR % 4 == 0) {
 #pragma unroll
-                for (int r = 0; r < NR; r += 4)
-                    *reinterpret_cast<float4 *>(x + r) = *reinterpret_cast<const float4 *>(xs + r);
-            } else {
+                    for (int r = 0; r < NR; r += 4)
+                        *reinterpret_cast<float4 *>(x + r) =
+                            *reinterpret_cast<const float4 *>(xs + r);
+                } else {
 #pragma unroll
-                for (int r = 0; r < NR; r += 2)
-                    *reinterpret_cast<float2 *>(x + r) = *reinterpret_cast<const float2 *>(xs + r);
-            }
+                    for (int r = 0; r < NR; r += 2)
+                        *reinterpret_cast<float2 *>(x + r) =
+                            *reinterpret_cast<const float2 *>(xs + r);
+                }
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const Float2 xx = pair(x[r], x[r]);
-                acc[r][0] = fma2(xx, q0, acc[r][0]);
-                acc[r][1] = fma2(xx, q1, acc[r][1]);
+                for (int r = 0; r < NR; r++) {
+                    const Float2 xx = pair(x[r], x[r]);
+                    acc[r][0] = fma2(xx, q0, acc[r][0]);
+                    acc[r][1] = fma2(xx, q1, acc[r][1]);
+                }
             }
         }
     }
