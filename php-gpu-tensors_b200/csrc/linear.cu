@@ -132,7 +132,7 @@ struct Plan {
     }
 };
 
-// Launches the layouts asked for so far.  Blocks for each in proportion to its
+// Launches the layouts asked for so far, two in one launch.  Blocks for each in proportion to its
 // work, one element vector a thread as far as 16 blocks an SM go.
 void flush_layouts(Plan &pl)
 {
@@ -377,11 +377,14 @@ cudaError_t launch_decode(const Plan &pl, const RaggedMaps &maps, RaggedParams &
     return cudaLaunchKernelEx(&cfg, kernel, maps, p, split);
 }
 
-// Few rows: at most half a tile's on average, or two tiles' when the pair
-// kernel would not occupy the GPU once.
+// Few rows: at most a quarter of a tile's on average, or two tiles' when the
+// pair kernel would not occupy the GPU once.  Measured on B200 (us, few rows /
+// pairs): one 4096 x 4096 weight, 16 rows 9.2 / 20.5, 64 rows 12.7 / 21.9, 128
+// rows 17.6 / 21.9, 256 rows 27.6 / 23.0; 32 experts of 2048 x 1024, 32 rows
+// 16.8 / 24.1, 1024 rows 35.6 / 30.5.
 bool few_rows(const PtgDevice &dev, long long pair_tiles, int rows, int groups)
 {
-    return rows <= kDecodeRows / 2 * static_cast<long long>(groups) ||
+    return rows <= kDecodeRows / 4 * static_cast<long long>(groups) ||
            (pair_tiles < dev.sms / 2 && rows <= kDecodeRows * 2ll * groups);
 }
 
@@ -591,7 +594,9 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
                       : static_cast<long long>((a.rows + span - 1) / span);
     };
     // tiles of fewer rows while the pairs are not all at work: they load more
-    // of the weight per row, but an idle pair loads nothing
+    // of the weight per row, but an idle pair loads nothing (us, so / in tiles of
+    // 256 rows: 256 x 4096 x 4096 23.1 / 26.4, 512 x 4096 x 1024 22.2 / 26.2,
+    // float32 4698 x 2816 x 102 149 / 171)
     p.span = kRaggedBN;
     long long bound = ft * row_tiles(p.span);
     const int path = ptg_path();
@@ -618,8 +623,10 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
 }
 
 // Parts that the rows of a group are cut into for dw: while its tiles leave
-// pairs idle, and every part keeps eight k-blocks on average.  A rule of the
-// sizes alone, since it also sizes the workspace.
+// pairs idle, and every part keeps eight k-blocks on average (us, so / in one
+// part: 16026 rows, 384 x 112 17.2 / 77.3; 4096 rows, 512 x 512 13.2 / 25.5; 8192
+// rows, 1024 x 1024 21.7 / 43.5).  A rule of the sizes alone, since it also sizes
+// the workspace.
 constexpr int kPairs = 74;
 
 int weight_parts(const PtgLinear &a)
@@ -724,8 +731,10 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
 
 // Whether a product runs on the CUDA cores: float32 ones below kSimtWork
 // multiply-adds, 16-bit ones below kSimtLayWork whose operands would have to
-// be laid out first.  The thread's kernel path decides first (2: CUDA cores,
-// 1 and 3: the tensor-core kernels).
+// be laid out first.  Measured on B200 (us, CUDA cores / three parts on the tensor
+// cores): 8 x 4096 x 4096 37 / 171, 64 x 1024 x 1024 20 / 37, 512 x 1024 x 1024
+// 50 / 49, 1024 x 1024 x 1024 90 / 52.  The thread's kernel path decides first (2:
+// CUDA cores, 1 and 3: the tensor-core kernels).
 constexpr double kSimtWork = 5.0e8;
 constexpr double kSimtLayWork = 5.0e7;
 constexpr double kExactGradient = 16384;
