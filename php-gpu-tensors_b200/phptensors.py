@@ -424,12 +424,8 @@ class CudaArray:
         [cols] arrays of this dtype or float32.  With save_stats the result is
         (y, mean, rstd), the float32 statistics layer_norm_backward takes."""
         _check_feed_forward("layer_norm", self, gamma, beta)
-        y = _result(self._shape, self._dtype, self)
-        lead = self._shape[:-1]
-        mean = rstd = None
-        if save_stats:
-            mean = _result(lead, "float32")
-            rstd = _result(lead, "float32", mean)
+        y = _result_like(self)
+        mean, rstd = _result_pair(self._shape[:-1]) if save_stats else (None, None)
         _raise_for(library().pt_layer_norm(
             _ref(self), _ref(gamma), _ref(beta), eps, _ref(y), _ptr(mean), _ptr(rstd),
             _raw_stream()))
@@ -492,6 +488,32 @@ def _result(shape, dtype, like=None):
     return self
 
 
+def _result_like(a):
+    """An uninitialised contiguous array of the shape and type of `a`."""
+    t = a._tensor
+    if t is None or not t.is_contiguous():
+        return _result(a._shape, a._dtype, a)
+    self = CudaArray.__new__(CudaArray)
+    self._tensor, self._flat = _torch().empty_like(t), None
+    self._dtype, self._offset = a._dtype, 0
+    self._shape, self._strides = a._shape, a._strides
+    return self
+
+
+def _result_pair(shape):
+    """Two uninitialised contiguous float32 arrays in one allocation."""
+    n = math.prod(shape)
+    flat = _torch().empty(2 * n, dtype=_TORCH_DTYPES["float32"], device="cuda")
+    strides = _contiguous_strides(shape)
+    pair = []
+    for offset in (0, n):
+        a = CudaArray.__new__(CudaArray)
+        a._tensor, a._flat, a._dtype, a._offset = None, flat, "float32", offset
+        a._shape, a._strides = list(shape), strides
+        pair.append(a)
+    return pair
+
+
 def _ref(a):
     """`a` as a pt_tensor argument; None as a null pointer."""
     return None if a is None else a._packed()
@@ -521,13 +543,12 @@ def layer_norm_backward(grad, x, gamma, mean, rstd, params=True):
         if s._dtype != "float32" or s._shape != lead or s._strides != _contiguous_strides(lead):
             raise InvalidArgumentException(
                 "layer norm statistics must be contiguous float32 arrays, one value a row")
-    dx = _result(x._shape, x._dtype, x)
+    dx = _result_like(x)
     dgamma = dbeta = work = None
     lib = library()
     size = ctypes.c_size_t(0)
     if params:
-        dgamma = _result([cols], "float32", mean)
-        dbeta = _result([cols], "float32", mean)
+        dgamma, dbeta = _result_pair([cols])
         size.value = lib.pt_layer_norm_backward_workspace(math.prod(lead), cols)
         work = _workspace(size.value)
     _raise_for(lib.pt_layer_norm_backward(
@@ -584,7 +605,7 @@ def _linear_backward(grad, x, weight, ends, pre, activation, bias, inputs, weigh
                      weight_grad_dtype):
     _check_feed_forward("linear_backward", grad, x, weight, pre)
     code = _activation_code(activation)
-    dx = _result(x._shape, x._dtype, x) if inputs else None
+    dx = _result_like(x) if inputs else None
     dw = None
     if weights:
         dw = _result(weight._shape, weight_grad_dtype or x._dtype,
