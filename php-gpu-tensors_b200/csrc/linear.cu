@@ -567,6 +567,7 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
     p.inner = inner;
     p.a_mn = transposed ? !w.cols_contiguous : w.cols_contiguous;
     p.passes = pl.passes;
+    p.parts = pl.parts;
     p.out_row = features;
     RaggedMaps maps;
     std::memset(&maps, 0, sizeof(maps));
@@ -654,6 +655,7 @@ cudaError_t weight_product(Plan &pl, const PtgLinear &a, const Rows &x, const Ro
     p.features = a.cols;
     p.cols = a.inner;
     p.passes = pl.passes;
+    p.parts = pl.parts;
     p.span = kRaggedBN;
     p.split = parts;
     p.idesc = instruction(a.dtype, true, true, 256);

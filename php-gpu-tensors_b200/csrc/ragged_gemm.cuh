@@ -47,7 +47,7 @@ struct RaggedParams {
     int inner;                // COLS: K
     int a_mn;                 // COLS: the weight's features are contiguous
     int a_chunks, b_chunks;   // that map walks 64-element chunks: one load per stage
-    int passes;               // CHUNKED: products of parts per k-block, 3 or 6
+    int passes, parts;        // CHUNKED: 6 products of 3 parts per k-block, or 3 of 2
     int span;                 // rows (INNER: columns) of a tile: 256, 128 or 64
     int split;                // INNER: parts of a group's rows, each with its own result
     int act;
@@ -81,11 +81,14 @@ struct RaggedMaps {
 
 constexpr int kMaxGroups = 2048;
 constexpr int kRaggedBN = 256;
-// A stage is two k-blocks: waits and commits hold up the thread that issues the
-// MMAs (8192^3 bfloat16: a commit to each CTA per k-block 776 us, one to both
-// 751), so there is one of each for eight MMAs.
-constexpr int kRaggedStages = 3;
+// A stage is two k-blocks, or CHUNKED one k-block in all its parts, so that each
+// part is loaded once for its two or three products.  Waits and commits hold up
+// the thread that issues the MMAs (8192^3 bfloat16: a commit to each CTA
+// per k-block 776 us, one to both 751, one for two k-blocks 724), so there is one
+// of each for eight MMAs or more.
+constexpr int ragged_stages(bool chunked) { return chunked ? 2 : 3; }
 constexpr int kStageKb = 2;
+constexpr int kMaxParts = 3;
 // Sixteen epilogue warps hide each other's latencies (TMEM, residual, stores);
 // CHUNKED ones keep a tile's sums in registers, 64 each.  Warps 0 and the last
 // issue the loads of the two operands, warp 1 the MMAs.
@@ -93,10 +96,12 @@ constexpr int kRaggedEpiWarps = 16;
 constexpr int kRaggedThreads = 32 * (3 + kRaggedEpiWarps);
 constexpr int kRaggedRowWarp = 2 + kRaggedEpiWarps;
 constexpr int kRaggedTile = 16384;                       // 128 rows x 64 of K, 16 bits
-constexpr int kRaggedKb = 2 * kRaggedTile;               // both operands of a k-block
-constexpr int kRaggedStage = kStageKb * kRaggedKb;
-constexpr int kRaggedRing = kRaggedStages * kRaggedStage;
-constexpr int kRaggedBars = 2 * kRaggedStages + 4 + 1;
+constexpr int kRaggedRing = 12 * kRaggedTile;
+constexpr int ragged_stage_bytes(bool chunked) { return kRaggedRing / ragged_stages(chunked); }
+static_assert(ragged_stage_bytes(false) == kStageKb * 2 * kRaggedTile &&
+                  ragged_stage_bytes(true) == kMaxParts * 2 * kRaggedTile,
+              "stages fill the ring");
+constexpr int kRaggedBars = 2 * ragged_stages(false) + 4 + 1;
 // the epilogue works on kGroup rows at a time: a warp's box of 32 features
 constexpr int kGroup = 16;
 constexpr int kRaggedBox = kGroup * 32 * 2;
@@ -106,7 +111,6 @@ constexpr int kRaggedTableOffset = kRaggedBarOffset + kRaggedBars * 8 + 24;
 constexpr int kRaggedSmem = kRaggedTableOffset + 2 * kMaxGroups * 4 + 1024;
 static_assert(kRaggedSmem <= 232448, "shared memory budget exceeded");
 constexpr int kChunkBlocks = 2;                          // k-blocks of 64 per chunk
-static_assert(kChunkBlocks % kStageKb == 0, "stages do not straddle chunks");
 constexpr int kFeatureBand = 8;                          // feature tiles walked per row tile
 
 // Index in RaggedMaps::rows of the smallest box that holds n rows.
@@ -429,7 +433,11 @@ template <typename T, bool INNER, bool CHUNKED>
 __global__ void __launch_bounds__(kRaggedThreads, 1)
     ragged_gemm_kernel(const __grid_constant__ RaggedMaps maps, const RaggedParams p)
 {
-    constexpr int S = kRaggedStages;
+    constexpr int S = ragged_stages(CHUNKED);
+    constexpr int kStageBytes = ragged_stage_bytes(CHUNKED);
+    // A and B of unit `sub` (k-block, or part) of a stage
+    constexpr int kASub = CHUNKED ? kRaggedTile : 2 * kRaggedTile, kBSub = kASub;
+    constexpr int kBOffset = CHUNKED ? kMaxParts * kRaggedTile : kRaggedTile;
     constexpr int kEpiWarps = kRaggedEpiWarps;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
@@ -482,7 +490,6 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     fill_groups(p.ends, p.groups, p.rows, p.span, table, table + kMaxGroups, total_end);
     const GroupTable groups = {table, table + kMaxGroups, p.groups, *total_end};
     const long long tiles = ragged_tiles<INNER>(p, groups);
-    const int passes = CHUNKED ? p.passes : 1;
 
     if (warp == 0 || warp == kRaggedRowWarp) {
         // ------------------------------------------------------------ producers (both CTAs)
@@ -503,14 +510,14 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                 const int box = INNER ? 0 : row_box(half);
                 const int b_boxes = p.b_chunks ? 2 : (half + 63) / 64;
                 const uint32_t bytes = kRaggedTile + (INNER ? b_boxes * 8192u : 2048u << box);
-                const int iters = r.k_blocks * passes;
+                const int units = CHUNKED ? r.k_blocks : (r.k_blocks + kStageKb - 1) / kStageKb;
                 const CUtensorMap *map = first ? &maps.a : INNER ? &maps.b : &maps.rows[box];
                 if (INNER && p.group_maps) {
                     map = p.group_maps + 2 * r.group + (first ? 0 : 1);
                     tensor_map_acquire(map);
                 }
-                for (int i = 0; i < iters; i += kStageKb) {
-                    const int count = min(kStageKb, iters - i);
+                for (int u = 0; u < units; u++) {
+                    const int count = CHUNKED ? p.parts : min(kStageKb, r.k_blocks - u * kStageKb);
                     if (!mbar_wait(&empty[stage], phase ^ 1, abort)) {
                         record_failure(abort, p.status, DEV_TIMEOUT_PRODUCER);
                         ok = false;
@@ -519,37 +526,34 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     if (first && rank == 0)
                         mbar_arrive_expect_tx(&full[stage], count * 2 * bytes);
                     const uint32_t full0 = full_leader + stage * 8;
+                    constexpr int kSubs = CHUNKED ? kMaxParts : kStageKb;
 #pragma unroll
-                    for (int sub = 0; sub < kStageKb; sub++) {
+                    for (int sub = 0; sub < kSubs; sub++) {
                         if (sub >= count)
                             break;
-                        int pa = 0, pb = 0, kb = i + sub;
-                        if (CHUNKED) {
-                            kb = (i + sub) / passes;
-                            pass_parts(passes, i + sub - kb * passes, pa, pb);
-                        }
-                        uint8_t *to = smem + stage * kRaggedStage + sub * kRaggedKb +
-                                      (first ? 0 : kRaggedTile);
-                        const int k = r.k0 + kb * 64;
+                        const int part = CHUNKED ? sub : 0;
+                        uint8_t *to = smem + stage * kStageBytes +
+                                      (first ? sub * kASub : kBOffset + sub * kBSub);
+                        const int k = r.k0 + (CHUNKED ? u : u * kStageKb + sub) * 64;
                         if (first) {
                             if (!INNER && !p.a_mn) {
-                                tma_load_5d_pair(to, map, full0, k, f, r.group, pa, 0);
+                                tma_load_5d_pair(to, map, full0, k, f, r.group, part, 0);
                             } else if (p.a_chunks) {
                                 tma_load_5d_pair(to, map, full0, 0, k, f >> 6,
-                                                 INNER ? pa : r.group, INNER ? 0 : pa);
+                                                 INNER ? part : r.group, INNER ? 0 : part);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < 2; j++)
                                     tma_load_5d_pair(to + j * 8192, map, full0, f + j * 64, k,
-                                                     INNER ? pa : r.group, INNER ? 0 : pa, 0);
+                                                     INNER ? part : r.group, INNER ? 0 : part, 0);
                             }
                         } else if (!INNER) {
-                            tma_load_5d_pair(to, map, full0, k, n, pb, 0, 0);
+                            tma_load_5d_pair(to, map, full0, k, n, part, 0, 0);
                         } else if (p.b_chunks) {
-                            tma_load_5d_pair(to, map, full0, 0, k, n >> 6, pb, 0);
+                            tma_load_5d_pair(to, map, full0, 0, k, n >> 6, part, 0);
                         } else {
                             for (int j = 0; j < b_boxes; j++)
-                                tma_load_5d_pair(to + j * 8192, map, full0, n + j * 64, k, pb, 0,
+                                tma_load_5d_pair(to + j * 8192, map, full0, n + j * 64, k, part, 0,
                                                  0);
                         }
                     }
@@ -586,15 +590,16 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             // descriptors of stage 0; a step of 16 bytes adds one to them
             const uint64_t a0 = smem_desc(smem_base, a_mn ? 8192 : 16, 1024, kLayoutSw128);
             const uint64_t b0 =
-                smem_desc(smem_base + kRaggedTile, INNER ? 8192 : 16, 1024, kLayoutSw128);
+                smem_desc(smem_base + kBOffset, INNER ? 8192 : 16, 1024, kLayoutSw128);
             const uint32_t a_step = (a_mn ? 16 * 128 : 32) / 16;
             constexpr uint32_t kBStep = (INNER ? 16 * 128 : 32) / 16;
             const uint32_t empty0 = smem_addr(empty);
             for (long long t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const uint32_t idesc = p.idesc | (static_cast<uint32_t>(r.n >> 3) << 17);
-                const int per = CHUNKED ? kChunkBlocks * passes : r.k_blocks;
-                int left = r.k_blocks * passes;
+                const int units = CHUNKED ? r.k_blocks : (r.k_blocks + kStageKb - 1) / kStageKb;
+                const int per = CHUNKED ? kChunkBlocks : units;
+                int left = units;
                 // a tile without k-blocks still hands over one (unused) chunk
                 do {
                     const int acc = static_cast<int>(chunk & 1);
@@ -609,24 +614,34 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kRaggedBN);
                     const int n = min(per, left);
                     left -= n;
-                    for (int i = 0; i < n; i += kStageKb) {
+                    for (int i = 0; i < n; i++) {
                         if (!mbar_wait(&full[stage], phase, abort)) {
                             record_failure(abort, p.status, DEV_TIMEOUT_MMA);
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t ad = a0 + stage * (kRaggedStage / 16);
-                        const uint64_t bd = b0 + stage * (kRaggedStage / 16);
-#pragma unroll
-                        for (int sub = 0; sub < kStageKb; sub++) {
-                            if (i + sub >= n)
-                                break;
+                        const uint64_t ad = a0 + stage * (kStageBytes / 16);
+                        const uint64_t bd = b0 + stage * (kStageBytes / 16);
+                        auto multiply = [&](uint64_t am, uint64_t bm, bool more) {
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                umma_f16_pair(d_tmem, ad + sub * (kRaggedKb / 16) + k * a_step,
-                                              bd + sub * (kRaggedKb / 16) + k * kBStep, idesc,
-                                              (i | sub | k) != 0);
+                                umma_f16_pair(d_tmem, am + k * a_step, bm + k * kBStep, idesc,
+                                              more || k != 0);
+                        };
+                        if constexpr (CHUNKED) {
+                            for (int q = 0; q < p.passes; q++) {
+                                int pa, pb;
+                                pass_parts(p.passes, q, pa, pb);
+                                multiply(ad + pa * (kASub / 16), bd + pb * (kBSub / 16),
+                                         (i | q) != 0);
+                            }
+                        } else {
+#pragma unroll
+                            for (int sub = 0; sub < kStageKb; sub++)
+                                if (i * kStageKb + sub < r.k_blocks)
+                                    multiply(ad + sub * (kASub / 16), bd + sub * (kBSub / 16),
+                                             (i | sub) != 0);
                         }
                         umma_commit_pair_both(empty0 + stage * 8);
                         if (++stage == S) {
