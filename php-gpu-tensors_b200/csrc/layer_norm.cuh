@@ -17,6 +17,12 @@
 // in shared memory and writes one partial row per parameter, and a second
 // launch adds the partial rows in order (no atomics: the result does not
 // depend on timing).
+//
+// On B200: 16384 x 4096 bfloat16 backwards 84 us and 5 us for the partial rows (403 MB
+// are 62 us at the copy rate; what is left is loads in flight: one row ahead
+// is what 128 registers hold, and rows brought ahead into shared memory
+// by bulk copies ran slower, 116 us, before the arithmetic was packed); 3001 x 1531
+// float32 forwards 16.5 us (5.6), of which a launch takes about five.
 #pragma once
 
 #include "ptx_sm100.cuh"

@@ -13,7 +13,9 @@
 // features x TR rows, four features x NR rows a thread, 32 of the inner axis
 // at a time through double-buffered shared memory, the next step's loads in
 // registers meanwhile.  The inner axis is split over a cluster of up to eight
-// blocks when the tiles are few; partial sums are added in rank order.
+// blocks when the tiles are few; partial sums are added in rank order.  On B200:
+// 8 x 4096 x 4096 float32 37 us (67 MB), 512 x 1024 x 1024 50 us, 4096 x 1024 x 1024
+// 290 us = 30 TFLOP/s (128 x 64 tiles, with 174 registers, were no faster).
 #pragma once
 
 #include "ragged_decode.cuh"

@@ -1,6 +1,6 @@
 // Feed-forward layers at tensor level (include/pt_feed_forward.h): argument
-// checks, the row views of strided tensors, and workspace layout, above the
-// launches of csrc/layer_norm.cu.
+// checks and the row views of strided tensors, above the launches of
+// csrc/layer_norm.cu and csrc/linear.cu.
 #include "pt_feed_forward.h"
 
 #include "internal.h"
