@@ -9,6 +9,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -132,17 +133,20 @@ struct Plan {
     }
 };
 
-// Launches the layouts asked for so far, two in one launch.  Blocks for each in proportion to its
-// work, one element vector a thread as far as 16 blocks an SM go.
+// Launches the layouts asked for so far, two in one launch, with blocks for
+// each in proportion to its work: two items a thread as far as five blocks an SM,
+// all that fit, go.
 void flush_layouts(Plan &pl)
 {
     if (pl.lays == 0 || !pl.run || !pl.ok())
         return;
     auto blocks = [&](const LayParams &p) {
-        const long long n = (p.rows * (p.ld / 8) + 255) / 256;
-        return static_cast<int>(std::min<long long>(n, pl.dev.sms * 16ll));
+        return (p.rows * (p.ld / 8) + 511) / 512;
     };
-    const int first = blocks(pl.lay[0]), second = pl.lays > 1 ? blocks(pl.lay[1]) : 0;
+    const long long n0 = blocks(pl.lay[0]), n1 = pl.lays > 1 ? blocks(pl.lay[1]) : 0;
+    const double fit = std::min(1.0, pl.dev.sms * 5.0 / std::max<double>(1.0, n0 + n1));
+    const int first = static_cast<int>(std::ceil(n0 * fit)),
+              second = static_cast<int>(std::ceil(n1 * fit));
     pl.lays = 0;
     if (first + second == 0)
         return;

@@ -58,17 +58,48 @@ __device__ __forceinline__ void load8(const T *row, long long inner, int c, int 
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void lay_out_one(const LayParams &p, long long r, int c)
-{
-    const T *row = static_cast<const T *>(p.src) + row_offset(p.rows_of, r);
+// Item i of a layout: eight elements of row i / (ld / 8).
+template <typename T, typename Index>
+struct LayItem {
     alignas(16) T v[8];
-    load8(row, p.inner, c, p.cols, p.vec, v);
-    uint16_t *out = p.out + r * p.ld + c;
-    if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(v);
-    else
-        store_parts(v, out, p.part, p.parts);
+    long long at;           // element offset of its place in the first part
+
+    __device__ __forceinline__ void load(const LayParams &p, Index i, Index per_row)
+    {
+        const Index r = i / per_row;
+        const int c = static_cast<int>(i - r * per_row) * 8;
+        load8(static_cast<const T *>(p.src) + row_offset(p.rows_of, r), p.inner, c, p.cols, p.vec,
+              v);
+        at = static_cast<long long>(r) * p.ld + c;
+    }
+    __device__ __forceinline__ void store(const LayParams &p) const
+    {
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint4 *>(p.out + at) = *reinterpret_cast<const uint4 *>(v);
+        else
+            store_parts(v, p.out + at, p.part, p.parts);
+    }
+};
+
+// The next item's loads are in flight while the current one is stored.
+template <typename T, typename Index>
+__device__ __forceinline__ void lay_out_items(const LayParams &p, Index first, Index step)
+{
+    const Index per_row = static_cast<Index>(p.ld / 8);
+    const Index n = static_cast<Index>(p.rows) * per_row;
+    if (first >= n)
+        return;
+    LayItem<T, Index> now, next;
+    now.load(p, first, per_row);
+    for (Index i = first;; i += step) {
+        const bool more = n - i > step;
+        if (more)
+            next.load(p, i + step, per_row);
+        now.store(p);
+        if (!more)
+            return;
+        now = next;
+    }
 }
 
 // One or two layouts in a launch: blocks below `first` make a, the others b.
@@ -80,22 +111,12 @@ __global__ void __launch_bounds__(256)
     grid_launch_dependents();
     const bool second = static_cast<int>(blockIdx.x) >= first;
     const LayParams &p = second ? b : a;
-    const int block = second ? blockIdx.x - first : blockIdx.x;
-    const int blocks = second ? gridDim.x - first : first;
-    const int per_row = p.ld / 8;
-    const long long total = p.rows * per_row;
-    if (total < (1ll << 31)) {
-        const unsigned n = static_cast<unsigned>(total), step = blocks * 256u;
-        for (unsigned i = block * 256u + threadIdx.x; i < n; i += step) {
-            const unsigned r = i / per_row;
-            lay_out_one<T>(p, r, static_cast<int>(i - r * per_row) * 8);
-        }
-    } else {
-        for (long long i = block * 256ll + threadIdx.x; i < total; i += blocks * 256ll) {
-            const long long r = i / per_row;
-            lay_out_one<T>(p, r, static_cast<int>(i - r * per_row) * 8);
-        }
-    }
+    const unsigned block = second ? blockIdx.x - first : blockIdx.x;
+    const unsigned blocks = second ? gridDim.x - first : first;
+    if (p.rows * (p.ld / 8) < (1ll << 31))
+        lay_out_items<T, unsigned>(p, block * 256u + threadIdx.x, blocks * 256u);
+    else
+        lay_out_items<T, long long>(p, block * 256ll + threadIdx.x, blocks * 256ll);
 }
 
 // A contiguous copy of a view whose rows have no single stride.

@@ -16,6 +16,10 @@ __device__ __forceinline__ long long row_offset(const RowView &v, long long r)
 {
     if (v.n == 1)
         return r * v.stride[0];
+    if (v.n == 2 && r < (1ll << 31)) {
+        const unsigned i = static_cast<unsigned>(r), e = v.ext[1], q = i / e;
+        return q * v.stride[0] + (i - q * e) * v.stride[1];
+    }
     long long off = 0;
     for (int d = v.n - 1; d >= 0; d--) {
         off += (r % v.ext[d]) * v.stride[d];
