@@ -275,57 +275,57 @@ __device__ __forceinline__ void pass_parts(int passes, int q, int &pa, int &pb)
     pb = (0x046 >> shift) & 3;
 }
 
-// residual of rows n0 .. n0 + kGroup - 1 (those below count) at this feature.
-template <typename T, typename Offset>
+// residual of rows n0 .. n0 + G - 1 (those below count) at this feature.
+template <typename T, typename Offset, int G>
 __device__ __forceinline__ void load_residual_at(const RaggedParams &p, int n0, int count,
-                                                 int feature, T (&r)[kGroup])
+                                                 int feature, T (&r)[G])
 {
     const T *base = static_cast<const T *>(p.residual);
     const Offset step = static_cast<Offset>(p.residual_row);
     const Offset at = static_cast<Offset>(n0) * step +
                       static_cast<Offset>(feature) * static_cast<Offset>(p.residual_inner);
-    if (count >= kGroup) {
+    if (count >= G) {
 #pragma unroll
-        for (int j = 0; j < kGroup; j++)
+        for (int j = 0; j < G; j++)
             r[j] = __ldg(base + (at + j * step));
     } else {
 #pragma unroll
-        for (int j = 0; j < kGroup; j++)
+        for (int j = 0; j < G; j++)
             if (j < count)
                 r[j] = __ldg(base + (at + j * step));
     }
 }
 
-template <typename T>
+template <typename T, int G>
 __device__ __forceinline__ void load_residual(const RaggedParams &p, int n0, int count,
-                                              int feature, T (&r)[kGroup])
+                                              int feature, T (&r)[G])
 {
     if (feature >= p.features)
         return;
     if (p.residual_small)
-        load_residual_at<T, uint32_t>(p, n0, count, feature, r);
+        load_residual_at<T, uint32_t, G>(p, n0, count, feature, r);
     else
-        load_residual_at<T, long long>(p, n0, count, feature, r);
+        load_residual_at<T, long long, G>(p, n0, count, feature, r);
 }
 
 // A group's values to their place: 32 lanes write 32 neighbouring features of
 // each row, through the warp's box and one TMA store (16-bit results; a lane's
 // shared-memory stores have constant offsets, where global ones would cost
 // address arithmetic each), or directly for the last rows of a group.
-template <typename T>
+template <typename T, int G>
 __device__ __forceinline__ void store_group(const RaggedParams &p, T *out, const CUtensorMap *map,
                                             uint8_t *box, int n0, int count, int f_warp,
-                                            int group, const float (&v)[kGroup])
+                                            int group, const float (&v)[G])
 {
     const int lane = threadIdx.x & 31;
-    if constexpr (sizeof(T) == 2) {
-        if (p.tma_store && count >= kGroup) {
+    if constexpr (sizeof(T) == 2 && G == kGroup) {
+        if (p.tma_store && count >= G) {
             if (lane == 0)
                 bulk_wait_group_read<0>();       // the box's last store has read it
             __syncwarp();
             T *mine = reinterpret_cast<T *>(box) + lane;
 #pragma unroll
-            for (int j = 0; j < kGroup; j++)
+            for (int j = 0; j < G; j++)
                 mine[j * 32] = from_float<T>(v[j]);
             fence_proxy_async_smem();
             __syncwarp();
@@ -341,13 +341,13 @@ __device__ __forceinline__ void store_group(const RaggedParams &p, T *out, const
         return;
     const long long ld = p.out_row;
     out += n0 * ld + feature;
-    if (count >= kGroup) {
+    if (count >= G) {
 #pragma unroll
-        for (int j = 0; j < kGroup; j++)
+        for (int j = 0; j < G; j++)
             out[j * ld] = from_float<T>(v[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < kGroup; j++)
+        for (int j = 0; j < G; j++)
             if (j < count)
                 out[j * ld] = from_float<T>(v[j]);
     }
@@ -355,10 +355,10 @@ __device__ __forceinline__ void store_group(const RaggedParams &p, T *out, const
 
 // Bias, activation and residual (r, already loaded) on the values v of rows
 // n0 .. and their stores.  Called by whole warps.
-template <typename T, bool INNER>
+template <typename T, bool INNER, int G>
 __device__ __forceinline__ void finish_group(const RaggedParams &p, const RaggedMaps &maps,
-                                             float (&v)[kGroup], int n0, int count, int f_warp,
-                                             int group, float bias, const T (&r)[kGroup], T *out,
+                                             float (&v)[G], int n0, int count, int f_warp,
+                                             int group, float bias, const T (&r)[G], T *out,
                                              T *pre, uint8_t *box)
 {
     constexpr bool kFast = sizeof(T) == 2;
@@ -367,19 +367,19 @@ __device__ __forceinline__ void finish_group(const RaggedParams &p, const Ragged
     if constexpr (!INNER) {
         const Float2 b2 = pair(bias, bias);
 #pragma unroll
-        for (int j = 0; j < kGroup; j += 2)
+        for (int j = 0; j < G; j += 2)
             split(add2(pair(v[j], v[j + 1]), b2), v[j], v[j + 1]);
         if (pre)
             store_group(p, pre, &maps.pre, box, n0, count, f_warp, 0, v);
         if (p.act != CUDA_MATMUL_EPILOGUE_NONE)
             with_activation(p.act, [&](auto act) {
 #pragma unroll
-                for (int j = 0; j < kGroup; j++)
+                for (int j = 0; j < G; j++)
                     v[j] = activate<act(), kFast>(v[j]);
             });
         if (p.residual) {
 #pragma unroll
-            for (int j = 0; j < kGroup; j++)
+            for (int j = 0; j < G; j++)
                 v[j] += to_float(r[j]);
         }
     }
@@ -434,6 +434,17 @@ __global__ void __launch_bounds__(256)
     }
     tensor_map_release();
 }
+
+__device__ __forceinline__ void tmem_ld_group(uint32_t taddr, uint32_t (&r)[16])
+{
+    tmem_ld_32x32b_x16(taddr, r);
+}
+__device__ __forceinline__ void tmem_ld_group(uint32_t taddr, uint32_t (&r)[8])
+{
+    tmem_ld_32x32b_x8(taddr, r);
+}
+__device__ __forceinline__ void tmem_wait_group(uint32_t (&r)[16]) { tmem_ld_wait_regs(r); }
+__device__ __forceinline__ void tmem_wait_group(uint32_t (&r)[8]) { tmem_ld_wait_regs8(r); }
 
 template <typename T, bool INNER, bool CHUNKED>
 __global__ void __launch_bounds__(kRaggedThreads, 1)
@@ -682,7 +693,9 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                      (INNER ? r.group * p.out_group + r.part * p.out_part : 0);
             T *pre = static_cast<T *>(p.pre);
             float bias = 0.0f;
-            T res[kGroup];
+            // (the chunks' sums leave room for smaller groups only)
+            constexpr int G = CHUNKED ? 8 : kGroup;
+            T res[G];
             if constexpr (!INNER) {
                 bias = load_bias<T>(p, r.group, feature);
                 if (!CHUNKED && p.residual && mine > 0)      // in flight while the products run
@@ -733,34 +746,34 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
                     }
                 }
                 if (c == chunks - 1) {
-                    uint32_t raw[kGroup];
+                    uint32_t raw[G];
                     if (mine > 0) {
-                        tmem_ld_32x32b_x16(t_acc, raw);
+                        tmem_ld_group(t_acc, raw);
                         if constexpr (CHUNKED && !INNER) {   // (the sums took the registers)
                             if (p.residual)
                                 load_residual(p, n0, r.n_end - n0, feature, res);
                         }
                     }
 #pragma unroll 1
-                    for (int h = 0; h < mine; h += kGroup) {
-                        float v[kGroup];
-                        T now[kGroup];
-                        tmem_ld_wait_regs(raw);
+                    for (int h = 0; h < mine; h += G) {
+                        float v[G];
+                        T now[G];
+                        tmem_wait_group(raw);
 #pragma unroll
-                        for (int j = 0; j < kGroup; j++) {
+                        for (int j = 0; j < G; j++) {
                             v[j] = __uint_as_float(raw[j]);
                             now[j] = res[j];
                         }
                         if (r.k_blocks == 0) {       // a sum over nothing
 #pragma unroll
-                            for (int j = 0; j < kGroup; j++)
+                            for (int j = 0; j < G; j++)
                                 v[j] = 0.0f;
                         }
-                        if (h + kGroup < mine) {
-                            tmem_ld_32x32b_x16(t_acc + h + kGroup, raw);
+                        if (h + G < mine) {
+                            tmem_ld_group(t_acc + h + G, raw);
                             if constexpr (!INNER) {
                                 if (p.residual)
-                                    load_residual(p, n0 + h + kGroup, r.n_end - (n0 + h + kGroup),
+                                    load_residual(p, n0 + h + G, r.n_end - (n0 + h + G),
                                                   feature, res);
                             }
                         }
