@@ -307,6 +307,8 @@ cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p
     if (pairs < 1)
         return cudaErrorInvalidConfiguration;
     p.status = pl.dev.status;
+    if (bound > 0x7fffffffll)
+        return cudaErrorInvalidValue;
     const long long n = std::max<long long>(1, std::min<long long>(bound, pairs));
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

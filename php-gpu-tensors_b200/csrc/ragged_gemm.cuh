@@ -207,42 +207,48 @@ struct RaggedTile {
     int k_blocks;
 };
 
+// Tile numbers are 32-bit: every role decodes each of its tiles, the ones that
+// issue loads and MMAs in a single thread, where 64-bit divisions would take
+// as long as some k-blocks.
 template <bool INNER>
-__device__ __forceinline__ long long ragged_tiles(const RaggedParams &p, const GroupTable &g)
+__device__ __forceinline__ unsigned ragged_tiles(const RaggedParams &p, const GroupTable &g)
 {
-    const long long ft = (p.features + 255) / 256;
+    const unsigned ft = (p.features + 255) / 256;
     if (INNER)
-        return ft * ((p.cols + p.span - 1) / p.span) * p.groups * p.split;
-    return ft * g.tiles[p.groups - 1];
+        return ft * static_cast<unsigned>((p.cols + p.span - 1) / p.span) * p.groups * p.split;
+    return ft * static_cast<unsigned>(g.tiles[p.groups - 1]);
 }
 
 template <bool INNER>
 __device__ __forceinline__ RaggedTile ragged_tile(const RaggedParams &p, const GroupTable &g,
-                                                  long long t)
+                                                  unsigned t)
 {
     RaggedTile r;
-    const int ft = (p.features + 255) / 256;
-    int rows_t, local;
+    const unsigned ft = (p.features + 255) / 256;
+    unsigned rows_t, local;
     if (INNER) {
         rows_t = (p.cols + p.span - 1) / p.span;
-        const int per = ft * rows_t;
-        const int unit = static_cast<int>(t / per);
-        local = static_cast<int>(t - static_cast<long long>(unit) * per);
-        r.group = unit / p.split;
+        const unsigned per = ft * rows_t, unit = t / per;
+        local = t - unit * per;
+        r.group = unit / static_cast<unsigned>(p.split);
         r.part = unit - r.group * p.split;
     } else {
-        r.group = find_group(g, static_cast<int>(t / ft));
-        const int before = r.group > 0 ? g.tiles[r.group - 1] : 0;
+        unsigned before = 0;
+        r.group = 0;
+        if (p.groups > 1) {
+            r.group = find_group(g, static_cast<int>(t / ft));
+            before = r.group > 0 ? g.tiles[r.group - 1] : 0;
+        }
         rows_t = g.tiles[r.group] - before;
-        local = static_cast<int>(t - static_cast<long long>(before) * ft);
+        local = t - before * ft;
     }
     // bands of kFeatureBand feature tiles, row tile by row tile: the clusters
     // at work at one time share their operands in L2
-    const int band = local / (kFeatureBand * rows_t);
-    const int wide = min(kFeatureBand, ft - band * kFeatureBand);
-    const int in_band = local - band * kFeatureBand * rows_t;
+    const unsigned band = local / (kFeatureBand * rows_t);
+    const unsigned wide = min(static_cast<unsigned>(kFeatureBand), ft - band * kFeatureBand);
+    const unsigned in_band = local - band * kFeatureBand * rows_t;
     const int nt = in_band / wide;
-    r.f0 = (band * kFeatureBand + in_band % wide) * 256;
+    r.f0 = (band * kFeatureBand + in_band - nt * wide) * 256;
     const int start = g.start[r.group], end = group_end(g, r.group);
     if (INNER) {
         // whole k-blocks for each part: only the group's last one may be ragged
@@ -473,8 +479,8 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
-    const long long cluster = blockIdx.x >> 1;
-    const long long nclusters = gridDim.x >> 1;
+    const unsigned cluster = blockIdx.x >> 1;
+    const unsigned nclusters = gridDim.x >> 1;
 
     if (warp == 0 && lane == 0) {
         if (INNER || p.inner > 0) {
@@ -506,7 +512,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
     grid_launch_dependents();
     fill_groups(p.ends, p.groups, p.rows, p.span, table, table + kMaxGroups, total_end);
     const GroupTable groups = {table, table + kMaxGroups, p.groups, *total_end};
-    const long long tiles = ragged_tiles<INNER>(p, groups);
+    const unsigned tiles = ragged_tiles<INNER>(p, groups);
 
     if (warp == 0 || warp == kRaggedRowWarp) {
         // ------------------------------------------------------------ producers (both CTAs)
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             uint32_t issued_mask = 0, parity_mask = 0;
             bool ok = true;
             const uint32_t full_leader = map_to_cta(smem_addr(full), 0);
-            for (long long t = cluster; ok && t < tiles; t += nclusters) {
+            for (unsigned t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const int half = r.n / 2;
                 const int f = r.f0 + static_cast<int>(rank) * 128;
@@ -611,7 +617,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
             const uint32_t a_step = (a_mn ? 16 * 128 : 32) / 16;
             constexpr uint32_t kBStep = (INNER ? 16 * 128 : 32) / 16;
             const uint32_t empty0 = smem_addr(empty);
-            for (long long t = cluster; ok && t < tiles; t += nclusters) {
+            for (unsigned t = cluster; ok && t < tiles; t += nclusters) {
                 const RaggedTile r = ragged_tile<INNER>(p, groups, t);
                 const uint32_t idesc = p.idesc | (static_cast<uint32_t>(r.n >> 3) << 17);
                 const int units = CHUNKED ? r.k_blocks : (r.k_blocks + kStageKb - 1) / kStageKb;
@@ -683,7 +689,7 @@ __global__ void __launch_bounds__(kRaggedThreads, 1)
         constexpr int kCols = kRaggedBN / (kEpiWarps / 4);
         long long chunk = 0;
         bool ok = true;
-        for (long long t = cluster; ok && t < tiles; t += nclusters) {
+        for (unsigned t = cluster; ok && t < tiles; t += nclusters) {
             const RaggedTile r = ragged_tile<INNER>(p, groups, t);
             const int f_warp = r.f0 + static_cast<int>(rank) * 128 + quad * 32;
             const int feature = f_warp + lane;
