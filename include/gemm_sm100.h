@@ -240,7 +240,8 @@ int cuda_matmul_epilogue_nd_launcher(
 /* Name of the kernel the last successful launch on this thread used, e.g.
  * "tc2-bf16-256x512", "tc2-bf16-256x256", "tc2-3xtf32-tmem-256x256",
  * "tc2-3xtf32-256x256", "tc-3xtf32-128x128",
- * "skinny-f32", "simt-f32"; "none" before any. */
+ * "skinny-f32", "simt-f32", "ragged2-bf16-256x256" (linear layers), "layer-norm";
+ * "none" before any. */
 const char *gemm_sm100_last_kernel(void);
 
 /* Grid size (CTAs), CTA size (threads) and cluster size of the last
@@ -260,7 +261,9 @@ void gemm_sm100_last_launch(int *grid, int *block, int *cluster);
  * products with a 16-bit result whenever the layout allows it (other
  * products as 3), 6 = the same kernel running every tile as two 256-column
  * halves (the form its last round of clusters takes when the automatic
- * choice splits it; for tests). */
+ * choice splits it; for tests).  The linear layers of pt_feed_forward.h take
+ * 1 as their few-row tensor-core kernel (dw: the pair kernel), 2 as their
+ * CUDA-core kernel, 3 as their pair kernel, and others as 0. */
 int gemm_sm100_set_path(int path);
 
 /* Reads (and with clear != 0 resets) the device status word of `device`:

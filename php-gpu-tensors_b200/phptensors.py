@@ -11,6 +11,10 @@ names, argument meaning and exceptions:
     cuda_tune_matmul                 src/cuda.c:211-290
     PhpTensors\\InvalidArgumentException / RuntimeException
 
+and, with no counterpart there, the feed-forward layers of
+include/pt_feed_forward.h: CudaArray.layer_norm, linear and grouped_linear with
+layer_norm_backward, linear_backward and grouped_linear_backward.
+
 Every product computed here runs on the GPU through the C ABI of
 include/gemm_sm100.h and include/pt_tensor.h (the C++ host layer
 pt_tensor_matmul_into dispatches to the launchers).  PyTorch is used only for
@@ -735,7 +739,8 @@ def set_kernel_path(path):
     tf32, strict float32, float32 x bf16), 4 few-column split-K kernel
     whenever N <= 32 and K >= 128, 5 the 2-CTA 256 x 512 kernel for 16-bit
     products with a 16-bit result (other products as 3), 6 the same kernel
-    running every tile as two 256-column halves."""
+    running every tile as two 256-column halves.  The linear layers take 1 as
+    their few-row kernel, 2 as their CUDA-core kernel, 3 as their pair kernel."""
     return library().gemm_sm100_set_path(
         {"auto": 0, "tensor-core": 1, "simt": 2, "tensor-core-pair": 3, "skinny": 4,
          "tensor-core-wide": 5, "tensor-core-wide-halves": 6}[path])
