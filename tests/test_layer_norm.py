@@ -175,6 +175,28 @@ def test_same_bits_again_and_on_another_stream():
         assert torch.equal(a, b)
 
 
+@gpu
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements: the last rows are those of a call on them alone."""
+    rows, cols = 270001, 8192
+    x = torch.randn(rows, cols, device="cuda", dtype=torch.bfloat16)
+    y, mean, rstd = arr(x).layer_norm(save_stats=True)
+    tail = x[rows - 3:].contiguous()
+    few, fm, fr = arr(tail).layer_norm(save_stats=True)
+    check_forward(tail, None, None, y.to_torch()[rows - 3:], mean.to_torch()[rows - 3:],
+                  rstd.to_torch()[rows - 3:], "bfloat16")
+    dx, dg, db = P.layer_norm_backward(y, arr(x), None, mean, rstd)
+    fx, _, _ = P.layer_norm_backward(arr(y.to_torch()[rows - 3:].contiguous()), arr(tail), None,
+                                     arr(mean.to_torch()[rows - 3:].contiguous()),
+                                     arr(rstd.to_torch()[rows - 3:].contiguous()))
+    assert torch.equal(dx.to_torch()[rows - 3:], fx.to_torch())
+    want = torch.zeros(cols, device="cuda").double()
+    for a in range(0, rows, 30000):
+        want += y.to_torch()[a:a + 30000].double().sum(0)
+    slack = (rows + 64) * E * y.to_torch()[:1000].double().abs().mean() * rows
+    assert torch.all((db.to_torch().double() - want).abs() <= slack)
+
+
 def _pt(shape, dtype):
     t = P.PtTensor()
     t.data, t.dtype, t.ndims = 4096, P.DTYPE_CODES[dtype], len(shape)

@@ -380,6 +380,55 @@ def test_same_bits_again_on_another_stream_and_in_a_graph(dtype, path):
         assert torch.equal(a, b) and torch.equal(a, k)
 
 
+@gpu
+@pytest.mark.parametrize("path", PATHS, indirect=True)
+@pytest.mark.parametrize("dtype", ALL)
+def test_broadcast_operands(dtype, path):
+    """One weight for all groups, one row for all rows, one upstream gradient:
+    strides of zero.  Each group still has its own gradient."""
+    ends = [40, 40, 100]
+    c = case(100, 72, 136, dtype, 17, groups=3)
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    spans = spans_of(ends, 100)
+    for name, shape in (("w", (3, 72, 136)), ("x", (100, 72)), ("grad", (100, 136)),
+                        ("pre", (100, 136)), ("res", (100, 136))):
+        c[name] = c[name][:1].expand(shape)
+    y = arr(c["x"]).grouped_linear(arr(c["w"]), at, arr(c["bias"]), "silu", arr(c["res"]))
+    check_forward(c, y.to_torch(), None, dtype, "silu", spans)
+    for act in ("silu", "none"):
+        out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at,
+                                        arr(c["pre"]), act)
+        check_backward(c, out, dtype, act, spans)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements: the last rows, and the sums over all of them."""
+    rows, inner, cols = 270001, 24, 8192
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, inner, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(inner, cols, generator=g, device="cuda") * 0.2).bfloat16()
+    c = {"x": x, "w": w}
+    y, pre = arr(x).linear(arr(w), None, "silu", save_pre=True)
+    tail = slice(rows - 300, rows)
+    check_forward(dict(c, x=x[tail]), y.to_torch()[tail], pre.to_torch()[tail], "bfloat16", "silu",
+                  [(0, 300)], bias=False, res=False)
+    grad, z = y.to_torch(), pre.to_torch()
+    dx, dw, db = P.linear_backward(y, arr(x), arr(w), pre, "silu")
+    k = dict(c, x=x[tail], grad=grad[tail], pre=z[tail])
+    want = P.linear_backward(arr(k["grad"].contiguous()), arr(k["x"].contiguous()), arr(w),
+                             arr(k["pre"].contiguous()), "silu")
+    assert torch.equal(dx.to_torch()[tail], want[0].to_torch())
+    sw, sb = torch.zeros(inner, cols, device="cuda").double(), torch.zeros(cols, device="cuda").double()
+    for a in range(0, rows, 30000):
+        dz = grad[a:a + 30000].double() * slope64(z[a:a + 30000].double(), "silu")
+        sw += x[a:a + 30000].double().T @ dz
+        sb += dz.sum(0)
+    # as wholes: dz's and the result's rounding, 2^-8 each
+    assert (dw.to_torch().double() - sw).norm() <= 2.0 ** -7 * sw.norm()
+    assert (db.to_torch().double() - sb).norm() <= 1e-5 * sb.norm()
+
+
 def _pt(shape, dtype):
     t = P.PtTensor()
     t.data, t.dtype, t.ndims = 4096, P.DTYPE_CODES[dtype], len(shape)
