@@ -265,9 +265,11 @@ __global__ void __launch_bounds__(512) layer_norm_long_kernel(const LayerNormPar
 }
 
 // Backwards: blocks walk the rows with a stride of the grid; the next row's
-// loads are issued before the current row's sums are joined.  On pairs of
-// columns, with n = x s - m s and dx = s a - s mean(a) - n s mean(a n), an
-// element costs about seven instructions; in scalar form (and as (x - m) s)
+// loads are issued before the current row's sums are joined.  The mean leaves x
+// before the product with s: x - m is nearly exact, where m s, rounded
+// on its own, would leave an error of the size of |m s| in every column of a
+// row that is far from zero.  On pairs of columns, with dx = s a - s mean(a) -
+// n s mean(a n), an element costs about eight instructions; in scalar form
 // issuing them, not memory, was the bound.
 template <typename T, int VB, int NV>
 __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const LayerNormParams p)
@@ -311,15 +313,15 @@ __global__ void __launch_bounds__(512) layer_norm_backward_kernel(const LayerNor
     // every group of the block makes the same number of steps
     for (long long base = first; base < p.rows; base += step, parity ^= 1) {
         const long long r = base + threadIdx.y;
-        const float rs = rstd, shift = -mean * rstd;
-        const Float2 rs2 = pair(rs, rs), shift2 = pair(shift, shift);
+        const float rs = rstd;
+        const Float2 rs2 = pair(rs, rs), minus = pair(-mean, -mean);
         Float2 n[P], a[P], s0 = zero, s1 = zero;
         unpack_pairs<T, VB>(rx, n);
         unpack_pairs<T, VB>(rg, a);
         fetch(r + step);
 #pragma unroll
         for (int k = 0; k < P; k++) {
-            n[k] = fma2(n[k], rs2, shift2);
+            n[k] = mul2(add2(n[k], minus), rs2);
             dg[k] = fma2(a[k], n[k], dg[k]);
             db[k] = add2(db[k], a[k]);
             a[k] = mul2(a[k], gam[k]);

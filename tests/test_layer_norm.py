@@ -231,3 +231,35 @@ def test_refusals():
     assert size.value == lib.pt_layer_norm_backward_workspace(4, 8) > 0
     assert lib.pt_layer_norm_backward(ref(_pt([4, 9], "float16")), ref(x), ref(g), 16, 16, ref(y),
                                       16, 16, None, ref(size), None) == P.PT_INVALID_ARGUMENT
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("rows,cols", [(5, 40), (9, 1024), (4, 1531), (3, 8192), (2, 20000)])
+@pytest.mark.parametrize("offset", [1e3, 1e4])
+def test_backward_of_rows_far_from_zero(dtype, rows, cols, offset):
+    """n = (x - mean) rstd from the statistics given: the difference of two
+    near floats is exact, so n is within 4 e of its own size however far the
+    row is from zero, a constant row (the last one) has n = 0, and the
+    tolerance holds no |x| rstd."""
+    x, grad, gamma, _ = make(rows, cols, dtype, cols, "plain")
+    x = (x.float() + offset).to(DT[dtype])
+    x[-1] = offset + 0.3
+    mean = x.double().mean(1).float()
+    mean[-1] = x[-1, 0].float()
+    d = x.double() - mean.double()[:, None]
+    rstd = ((d.square().mean(1) + EPS) ** -0.5).float()
+    dx, dg, db = P.layer_norm_backward(arr(grad), arr(x), arr(gamma), arr(mean), arr(rstd))
+    r = rstd.double()[:, None]
+    n = d * r
+    assert not n[-1].any()
+    a = grad.double() * gamma.double()
+    want = r * (a - a.mean(1, keepdim=True) - n * (a * n).mean(1, keepdim=True))
+    ma, mn = a.abs().mean(1, keepdim=True), (a * n).abs().mean(1, keepdim=True)
+    tol = UNIT[dtype] * want.abs() + 64 * E * r * (a.abs() + ma + n.abs() * mn)
+    if dtype == "float16":
+        tol += 2.0 ** -25
+    assert torch.all((dx.to_torch().double() - want).abs() <= tol)
+    terms = grad.double() * n
+    assert torch.all((dg.to_torch().double() - terms.sum(0)).abs()
+                     <= (rows + 64) * E * terms.abs().sum(0))
