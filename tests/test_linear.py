@@ -474,3 +474,48 @@ def test_refusals():
     assert size.value >= 3 * 2 * (4 * 8 + 8 * 16)
     with pytest.raises(P.InvalidArgumentException):
         P._activation_code("swish")
+
+
+TAIL = [-9.5, -8.0, -7.25, -6.0, -5.0, -4.0, -3.5, -3.0, -1.0, -0.25, 0.25, 1.0, 3.0, 6.0, 9.0]
+
+
+@gpu
+@pytest.mark.parametrize("path", PATHS[1:], indirect=True)
+@pytest.mark.parametrize("dtype", ALL)
+def test_gelu_keeps_its_digits_in_the_tail(dtype, path):
+    """z P(z) relative to itself, through a product that is z exactly.  float16
+    values below its spacing aside, what enters is the exponential and the
+    argument's roundings, z^2 / 2 times a few e, the tail's fit (2^-17, 16-bit
+    results) and the result's rounding."""
+    z = torch.tensor(TAIL, device="cuda", dtype=DT[dtype])
+    x = torch.zeros(len(TAIL), 64, device="cuda", dtype=DT[dtype])
+    x[:, 3] = z
+    w = torch.zeros(64, 72, device="cuda", dtype=DT[dtype])
+    w[3] = 1
+    y = arr(x).linear(arr(w), activation="gelu").to_torch().double()
+    z = z.double()
+    want = z * 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+    tol = UNIT[dtype] + (2 * z * z + 16) * 2.0 ** -24 + (0 if dtype == "float32" else 2.0 ** -17)
+    assert torch.all((y - want[:, None]).abs() <= (tol * want.abs() + TINY[dtype])[:, None])
+
+
+def slope_of(act, z, dtype):
+    """act'(z) in float32: dbias of one row whose upstream gradient is one."""
+    n = z.numel()
+    one = torch.ones(1, n, device="cuda", dtype=DT[dtype])
+    x, w = (torch.zeros(s, device="cuda", dtype=DT[dtype]) for s in ((1, 8), (8, n)))
+    return P.linear_backward(arr(one), arr(x), arr(w), arr(z[None]), act, inputs=False,
+                             weights=False)[2].to_torch().double()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+def test_gelu_slope_keeps_its_digits_in_the_tail(dtype):
+    """P(z) + z p(z), relative to its terms, of the same sources as above."""
+    z = torch.tensor(TAIL, device="cuda", dtype=DT[dtype])
+    v = z.double()
+    p = torch.exp(-0.5 * v * v) * (0.5 / math.pi) ** 0.5
+    cdf = 0.5 * torch.special.erfc(-v * 0.5 ** 0.5)
+    tol = (2 * v * v + 16) * 2.0 ** -24 + (0 if dtype == "float32" else 2.0 ** -17)
+    assert torch.all((slope_of("gelu", z, dtype) - (cdf + v * p)).abs()
+                     <= tol * (cdf + (v * p).abs()))
