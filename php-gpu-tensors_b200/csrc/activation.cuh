@@ -82,12 +82,13 @@ __device__ __forceinline__ float activation_slope(float z)
 {
     if constexpr (ACT == CUDA_MATMUL_EPILOGUE_RELU)
         return z > 0.0f ? 1.0f : 0.0f;
-    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_TANH) {
-        const float t = tanhf(z);
-        return fmaf(-t, t, 1.0f);
-    } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SIGMOID) {
-        const float s = divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-z));
-        return s * (1.0f - s);
+    else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_TANH || ACT == CUDA_MATMUL_EPILOGUE_SIGMOID) {
+        // even functions of z, from the exponential that is at most one: 1 - tanh^2
+        // = 4 e / (1 + e)^2 with e = e^(-2 |z|), and s (1 - s) = e / (1 + e)^2 with
+        // e^(-|z|); the differences would cancel in the tails
+        constexpr bool kTanh = ACT == CUDA_MATMUL_EPILOGUE_TANH;
+        const float e = exp_of<FAST>(fabsf(z) * (kTanh ? -2.0f : -1.0f));
+        return divide<FAST>(kTanh ? 4.0f * e : e, (1.0f + e) * (1.0f + e));
     } else if constexpr (ACT == CUDA_MATMUL_EPILOGUE_SILU) {
         const float s = divide<FAST>(1.0f, 1.0f + exp_of<FAST>(-z));
         return s * fmaf(z, 1.0f - s, 1.0f);

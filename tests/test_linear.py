@@ -519,3 +519,16 @@ def test_gelu_slope_keeps_its_digits_in_the_tail(dtype):
     tol = (2 * v * v + 16) * 2.0 ** -24 + (0 if dtype == "float32" else 2.0 ** -17)
     assert torch.all((slope_of("gelu", z, dtype) - (cdf + v * p)).abs()
                      <= tol * (cdf + (v * p).abs()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+def test_tanh_and_sigmoid_slopes_keep_their_digits_in_the_tail(dtype):
+    """1 - tanh^2 and s (1 - s) relative to themselves: an exponential of at most
+    2 |z|, within (2.4 |z| + 4) units of 2^-23 (16-bit operands), and a few
+    roundings."""
+    z = torch.tensor(TAIL, device="cuda", dtype=DT[dtype])
+    v = z.double()
+    tol = (5 * v.abs() + 32) * 2.0 ** -24
+    for act, want in (("tanh", torch.cosh(v) ** -2), ("sigmoid", 0.25 * torch.cosh(0.5 * v) ** -2)):
+        assert torch.all((slope_of(act, z, dtype) - want).abs() <= tol * want), act
