@@ -82,10 +82,13 @@ int pt_linear(const pt_tensor *x, const pt_tensor *w, const int *ends, const pt_
  *     dbias = column sums of dz, float32 [N] ([E, N])
  * each unless NULL; the residual's gradient is grad itself.  pre may be NULL
  * for CUDA_MATMUL_EPILOGUE_NONE.  For 16-bit operands dz is rounded to their
- * type before the two products (dbias is summed before that; where dz has no
- * more than 16384 elements it stays in float32); without an activation grad is
- * used as it is.  Rows of no group take no part, and their
- * dx is zero; a group without rows has a gradient of zero. */
+ * type before the two products, except where these run on the CUDA cores: where
+ * dz has no more than 16384 elements (unless gemm_sm100_set_path chose 1 or 3), for
+ * small products of operands that would have to be laid out, and where path 2
+ * was chosen.  There it stays in float32, whatever type dw is wanted in.
+ * dbias is summed before the rounding; without an activation grad is used as it is.
+ * Rows of no group take no part, and their dx is zero; a group without rows has
+ * a gradient of zero. */
 int pt_linear_backward(const pt_tensor *grad, const pt_tensor *x, const pt_tensor *w,
                        const int *ends, const pt_tensor *pre, int activation,
                        const pt_tensor *dx, const pt_tensor *dw, float *dbias, void *workspace,

@@ -262,6 +262,14 @@ const char *kernel_name(int family, int dtype)
 // ------------------------------------------------------------ products
 constexpr int kMaxDevices = 64;
 
+// The thread's kernel path as far as these layers have it: 1 few rows, 2 CUDA
+// cores, 3 pairs; the others are the matmul's own and leave the choice automatic.
+int layer_path()
+{
+    const int path = ptg_path();
+    return path <= 3 ? path : 0;
+}
+
 // CTA pairs of `kernel` that fit the device at one time; raises its
 // shared-memory limit on the first call on a device.  0 on failure.  (The
 // kernel is a template argument: the kernels share one function type.)
@@ -499,7 +507,7 @@ cudaError_t simt_product(Plan &pl, const PtgLinear &a, const Plain &x, bool tran
     return launch_simt<false>(pl, s, a.dtype, x.f32);
 }
 
-// dw as weight_product() does it; the result has the operands' type.
+// dw as weight_product() does it.
 cudaError_t simt_weight_product(Plan &pl, const PtgLinear &a, const Plain &x,
                                 const Plain &dz)
 {
@@ -514,6 +522,7 @@ cudaError_t simt_weight_product(Plan &pl, const PtgLinear &a, const Plain &x,
     s.p.out = a.dw;
     s.p.out_row = a.cols;
     s.p.out_group = static_cast<long long>(a.inner) * a.cols;
+    s.out_f32 = a.dw_dtype == DTYPE_FLOAT32;
     s.a = x.p;
     s.a_row = x.inner;
     s.a_inner = x.row;
@@ -606,7 +615,7 @@ cudaError_t product(Plan &pl, const PtgLinear &a, const Rows &x, const Weight &w
     // float32 4698 x 2816 x 102 149 / 171)
     p.span = kRaggedBN;
     long long bound = ft * row_tiles(p.span);
-    const int path = ptg_path();
+    const int path = layer_path();
     const bool few = a.dtype != DTYPE_FLOAT32 && path != 3 &&
                      (path == 1 || few_rows(pl.dev, bound, a.rows, a.groups));
     p.idesc = instruction(a.dtype, p.a_mn, false, few ? 128 : 256);
@@ -745,11 +754,20 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
 // CUDA cores, 1 and 3: the tensor-core kernels).
 constexpr double kSimtWork = 5.0e8;
 constexpr double kSimtLayWork = 5.0e7;
+
+// Elements of dz up to which 16-bit operands with an activation keep it in
+// float32, and so take the CUDA cores.  Rounding dz puts the gradients at 1.2 units
+// of roundoff from float64 in the norm, at any size, instead of 0.85; in
+// sums of a few terms nothing averages out (one row: dw's worst element 45
+// instead of 24 units of its rms).  us, float32 / rounded on the tensor cores, both
+// gradients: 64 x 1024 x 256 28 / 33, 16 x 1024 x 1024 28 / 20, 16 x 4096 x 1024 62 / 22,
+// 4 x 4096 x 4096 155 / 29: up to here the exact form costs some 20 us for layers
+// of ordinary width, and a wide layer's few rows pay in proportion to its weight.
 constexpr double kExactGradient = 16384;
 
 bool on_cuda_cores(const PtgLinear &a, bool lay)
 {
-    const int path = ptg_path();
+    const int path = layer_path();
     if (path == 1 || path == 3)
         return false;
     const double work = static_cast<double>(a.rows) * a.inner * a.cols;
@@ -849,8 +867,7 @@ void backward(Plan &pl, const PtgLinear &a)
     // roundings to 16 bits would not average out in the products
     const bool exact = a.dtype != DTYPE_FLOAT32 && active &&
                        static_cast<double>(a.rows) * a.cols <= kExactGradient;
-    const bool simt = (on_cuda_cores(a, lay) || (exact && ptg_path() == 0)) &&
-                      (!a.dw || a.dw_dtype == a.dtype);
+    const bool simt = on_cuda_cores(a, lay) || (exact && layer_path() == 0);
     const size_t partial_rows = a.rows / kSlopeRows + std::min(a.groups, a.rows);
     float *partial = a.dbias ? static_cast<float *>(pl.ws.take(partial_rows * a.cols * 4)) : nullptr;
 

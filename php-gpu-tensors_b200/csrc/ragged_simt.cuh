@@ -28,6 +28,7 @@ struct RaggedSimtParams {
     long long a_row, a_inner;           // element strides of A
     long long b_inner, b_col, b_group;  // and of B
     int split;
+    int out_f32;                        // INNER: the result is float32 whatever T is
 };
 
 constexpr int kSimtStep = 32;           // of the inner axis at a time
@@ -216,6 +217,12 @@ __global__ void __launch_bounds__(kSimtThreads) ragged_simt_kernel(const RaggedS
                 v = partial[e];
             }
             const long long at = static_cast<long long>(row) * p.out_row + feature;
+            if constexpr (INNER && sizeof(T) == 2) {
+                if (s.out_f32) {
+                    static_cast<float *>(p.out)[group * p.out_group + at] = v;
+                    continue;
+                }
+            }
             if constexpr (!INNER) {
                 v += load_bias<T>(p, group, feature);
                 if (pre)

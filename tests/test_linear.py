@@ -532,3 +532,37 @@ def test_tanh_and_sigmoid_slopes_keep_their_digits_in_the_tail(dtype):
     tol = (5 * v.abs() + 32) * 2.0 ** -24
     for act, want in (("tanh", torch.cosh(v) ** -2), ("sigmoid", 0.25 * torch.cosh(0.5 * v) ** -2)):
         assert torch.all((slope_of(act, z, dtype) - want).abs() <= tol * want), act
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [64, 65])
+def test_float32_weight_gradient_with_an_activation(dtype, rows):
+    """On both sides of 16384 elements of dz: asking for dw in float32 changes
+    dw's rounding alone, and a kernel path that is none of the linear layers'
+    changes nothing."""
+    ends = [20, 20, rows - 1]
+    c = case(rows, 96, 256, dtype, 31, groups=3)
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+
+    def back(path, dw=None):
+        before = P.set_kernel_path(path)
+        try:
+            return P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at,
+                                             arr(c["pre"]), "gelu", weight_grad_dtype=dw)
+        finally:
+            P.library().gemm_sm100_set_path(before)
+    want = back("auto")
+    check_backward(c, want, dtype, "gelu", spans_of(ends, rows))
+    for path in ("auto", "skinny", "tensor-core-wide"):
+        for dw in (None, "float32"):
+            got = back(path, dw)
+            for a, b in zip(want, got):
+                assert torch.equal(a.to_torch(), b.to_torch().to(a.to_torch().dtype)), (path, dw)
+            if dw:
+                check_backward(c, got, dtype, "gelu", spans_of(ends, rows), dw_dtype="float32")
+    # the CUDA-core path stays what was asked for
+    got = back("simt", "float32")
+    assert P.cuda_get_backend_info()["kernel"] == "ragged-simt-" + {"bfloat16": "bf16"}.get(
+        dtype, "f16")
+    check_backward(c, got, dtype, "gelu", spans_of(ends, rows), dw_dtype="float32")
