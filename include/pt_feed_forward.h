@@ -12,7 +12,8 @@
  * Operands are float32, float16 or bfloat16, all of one type unless said
  * otherwise; sums, statistics and activations are computed in float32 and a
  * result is rounded once.  float32 products follow the thread's precision
- * mode (cuda_blas_set_precision).
+ * mode (cuda_blas_set_precision).  Columns, inner elements and the linear layers'
+ * rows number fewer than 2^31 - 1024 each; offsets are 64-bit.
  */
 #ifndef PT_FEED_FORWARD_H
 #define PT_FEED_FORWARD_H

@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(256) layer_norm_param_long_kernel(const LayerN
     }
     float *part = p.partial + static_cast<long long>(blockIdx.y) * 2 * p.cols;
     part[c] = dg;
-    part[p.cols + c] = db;
+    part[static_cast<long long>(p.cols) + c] = db;
 }
 
 // out[s][c] = sum over n partial rows of partial[k][s * cols + c], in the

@@ -26,6 +26,10 @@ int submitted(cudaError_t err, const char *what)
     return ptg_fail(PT_RUNTIME, text);
 }
 
+// Extents that the kernels walk with 32-bit indexes, which step up to a tile past
+// the end before they are compared with it.
+constexpr int kMaxExtent = 2147483647 - 1024;
+
 bool float_type(int dtype)
 {
     return dtype == DTYPE_FLOAT32 || dtype == DTYPE_FLOAT16 || dtype == DTYPE_BFLOAT16;
@@ -130,6 +134,8 @@ PT_API int pt_layer_norm(const pt_tensor *x, const pt_tensor *gamma, const pt_te
     const int cols = last(x);
     if (cols < 1)
         return invalid("layer norm requires at least one column");
+    if (cols > kMaxExtent)
+        return invalid("layer norm takes fewer than 2^31 - 1024 columns");
     if (!parameter(gamma, x, cols) || !parameter(beta, x, cols))
         return invalid("layer norm gamma and beta must be [cols] vectors of the tensor's type or "
                        "float32");
@@ -179,6 +185,8 @@ PT_API int pt_layer_norm_backward(const pt_tensor *grad, const pt_tensor *x,
     const int cols = last(x);
     if (cols < 1)
         return invalid("layer norm requires at least one column");
+    if (cols > kMaxExtent)
+        return invalid("layer norm takes fewer than 2^31 - 1024 columns");
     if (!parameter(gamma, x, cols))
         return invalid("layer norm gamma and beta must be [cols] vectors of the tensor's type or "
                        "float32");
@@ -259,8 +267,8 @@ int layer(const pt_tensor *x, const pt_tensor *w, const int *ends, int activatio
     const long long rows = row_count(x);
     if (a->groups < 1 || a->groups > PT_MAX_GROUPS)
         return invalid("a grouped linear layer takes 1 to 2048 groups");
-    if (rows > 2147483647ll - 1024)
-        return invalid("linear layers take fewer than 2^31 - 1024 rows");
+    if (rows > kMaxExtent || a->inner > kMaxExtent || a->cols > kMaxExtent)
+        return invalid("linear layers take fewer than 2^31 - 1024 rows, inner elements and columns");
     if (!row_view(x, &a->xv))
         return invalid("linear layer cannot merge the tensor's leading axes");
     a->dtype = x->dtype;

@@ -263,3 +263,17 @@ def test_backward_of_rows_far_from_zero(dtype, rows, cols, offset):
     terms = grad.double() * n
     assert torch.all((dg.to_torch().double() - terms.sum(0)).abs()
                      <= (rows + 64) * E * terms.abs().sum(0))
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    """Rows stay 1024 columns below 2^31: a thread's column steps past the end
+    before it compares.  Refused before any CUDA call."""
+    lib, ref = P.library(), ctypes.byref
+    x = _pt([1, 2 ** 31 - 1024], "bfloat16")
+    assert lib.pt_layer_norm(ref(x), None, None, 1e-5, ref(x), None, None,
+                             None) == P.PT_INVALID_ARGUMENT
+    assert b"2^31" in lib.pt_last_error()
+    size = ctypes.c_size_t(0)
+    assert lib.pt_layer_norm_backward(ref(x), ref(x), None, 16, 16, ref(x), 16, 16, None,
+                                      ref(size), None) == P.PT_INVALID_ARGUMENT
+    assert b"2^31" in lib.pt_last_error()

@@ -566,3 +566,19 @@ def test_float32_weight_gradient_with_an_activation(dtype, rows):
     assert P.cuda_get_backend_info()["kernel"] == "ragged-simt-" + {"bfloat16": "bf16"}.get(
         dtype, "f16")
     check_backward(c, got, dtype, "gelu", spans_of(ends, rows), dw_dtype="float32")
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    """Column and inner counts stay 1024 below 2^31, as row counts do: loops and
+    tiles may step past the end before they compare.  Refused before any CUDA
+    call; no memory of these sizes is touched."""
+    lib, ref = P.library(), ctypes.byref
+    size = ctypes.c_size_t(0)
+    big = 2 ** 31 - 1024
+    for x, w, y in (([1, 8], [8, big], [1, big]), ([1, big], [big, 1], [1, 1])):
+        x, w, y = (_pt(s, "bfloat16") for s in (x, w, y))
+        assert lib.pt_linear(ref(x), ref(w), None, None, 0, None, ref(y), None, None, ref(size),
+                             None) == P.PT_INVALID_ARGUMENT
+        assert lib.pt_linear_backward(ref(y), ref(x), ref(w), None, None, 0, ref(x), ref(w), None,
+                                      None, ref(size), None) == P.PT_INVALID_ARGUMENT
+        assert b"2^31" in lib.pt_last_error()
