@@ -256,25 +256,45 @@ class CudaArray:
     def __init__(self, storage, shape, strides=None, offset=0, dtype="float32"):
         _check_dtype(dtype)
         self._flat = storage               # 1-D torch tensor of the dtype
-        self._tensor = None
+        self._tensor = self._memory = None
         self._shape = [int(d) for d in shape]
         self._strides = [int(s) for s in (strides if strides is not None
                                           else _contiguous_strides(self._shape))]
         self._offset = int(offset)
         self._dtype = dtype
 
+    def _same_memory(self):
+        """Whether the wrapped tensor still has the memory that was wrapped."""
+        return (self._memory is None
+                or self._tensor.untyped_storage()._cdata == self._memory._cdata)
+
+    def _wrapped(self):
+        """A torch tensor of this array's memory, shape and strides: the wrapped
+        one while it still has them, as its owner may give it others
+        (`tensor.data = ...`, transpose_)."""
+        t = self._tensor
+        if self._memory is not None and not (
+                self._same_memory() and t.storage_offset() == self._offset
+                and list(t.shape) == self._shape and list(t.stride()) == self._strides):
+            t = _torch().empty(0, dtype=_TORCH_DTYPES[self._dtype], device=self._memory.device)
+            t.set_(self._memory, self._offset, self._shape, self._strides)
+            self._tensor, self._memory = t, None
+        return t
+
     @property
     def _storage(self):
         """The whole storage as a 1-D torch tensor (of a wrapped tensor made
         when it is first asked for)."""
         if self._flat is None:
-            t = self._tensor
+            t = self._wrapped()
             n = t.untyped_storage().nbytes() // t.element_size()
             self._flat = _torch().as_strided(t, (n,), (1,), 0)
         return self._flat
 
     def _address(self):
         """Device address of the first element."""
+        if self._memory is not None:
+            return self._memory.data_ptr() + self._offset * ELEMENT_BYTES[self._dtype]
         if self._tensor is not None:
             return self._tensor.data_ptr()
         return self._flat.data_ptr() + self._offset * ELEMENT_BYTES[self._dtype]
@@ -300,12 +320,18 @@ class CudaArray:
 
     @classmethod
     def from_torch(cls, tensor, dtype=None):
-        """Wraps a CUDA torch tensor view without copying (storage offset kept)."""
-        _torch()
+        """Wraps a CUDA torch tensor view without copying (storage offset kept).
+        The array keeps the memory, the shape and the strides of this moment,
+        whatever the tensor object is given later."""
+        if _TORCH is None:
+            _torch()
         self = cls.__new__(cls)
-        self._dtype = dtype or _DTYPE_NAMES[tensor.dtype]
-        _check_dtype(self._dtype)
-        self._tensor, self._flat = tensor, None
+        if dtype is None:
+            self._dtype = _DTYPE_NAMES[tensor.dtype]
+        else:
+            _check_dtype(dtype)
+            self._dtype = dtype
+        self._tensor, self._flat, self._memory = tensor, None, tensor.untyped_storage()
         self._shape, self._strides = list(tensor.shape), list(tensor.stride())
         self._offset = tensor.storage_offset()
         return self
@@ -452,9 +478,9 @@ class CudaArray:
 
     # ---------------------------------------------------------- export
     def to_torch(self):
-        """A torch view of this array (no copy)."""
+        """A new torch view of this array (no copy)."""
         if self._tensor is not None:
-            return self._tensor
+            return self._wrapped()[...]
         return self._storage.as_strided(self._shape, self._strides, self._offset)
 
     def toArray(self):
@@ -483,11 +509,12 @@ def _result(shape, dtype, like=None):
     """An uninitialised contiguous array; `like`, an array of the same type,
     saves torch's own argument handling."""
     self = CudaArray.__new__(CudaArray)
-    if like is not None and like._tensor is not None:
-        t = like._tensor.new_empty(shape)
+    t = None if like is None else like._tensor
+    if t is not None and like._same_memory() and t.dtype == _TORCH_DTYPES[dtype]:
+        t = t.new_empty(shape)
     else:
         t = _torch().empty(shape, dtype=_TORCH_DTYPES[dtype], device="cuda")
-    self._tensor, self._flat, self._dtype, self._offset = t, None, dtype, 0
+    self._tensor, self._flat, self._memory, self._dtype, self._offset = t, None, None, dtype, 0
     self._shape, self._strides = list(shape), list(t.stride())
     return self
 
@@ -495,10 +522,10 @@ def _result(shape, dtype, like=None):
 def _result_like(a):
     """An uninitialised contiguous array of the shape and type of `a`."""
     t = a._tensor
-    if t is None or not t.is_contiguous():
+    if t is None or not a._same_memory() or list(t.shape) != a._shape or not t.is_contiguous():
         return _result(a._shape, a._dtype, a)
     self = CudaArray.__new__(CudaArray)
-    self._tensor, self._flat = _torch().empty_like(t), None
+    self._tensor, self._flat, self._memory = _torch().empty_like(t), None, None
     self._dtype, self._offset = a._dtype, 0
     self._shape, self._strides = a._shape, a._strides
     return self
@@ -512,8 +539,8 @@ def _result_pair(shape):
     pair = []
     for offset in (0, n):
         a = CudaArray.__new__(CudaArray)
-        a._tensor, a._flat, a._dtype, a._offset = None, flat, "float32", offset
-        a._shape, a._strides = list(shape), strides
+        a._tensor, a._flat, a._memory = None, flat, None
+        a._dtype, a._offset, a._shape, a._strides = "float32", offset, list(shape), strides
         pair.append(a)
     return pair
 
