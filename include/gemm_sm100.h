@@ -245,8 +245,9 @@ int cuda_matmul_epilogue_nd_launcher(
 const char *gemm_sm100_last_kernel(void);
 
 /* Grid size (CTAs), CTA size (threads) and cluster size of the last
- * tensor-core or few-column launch on this thread (0 before any); any pointer
- * may be NULL. */
+ * tensor-core, few-column or feed-forward launch on this thread (0 before any);
+ * of a feed-forward call's launches the last product's, or the first where there is
+ * no product.  Any pointer may be NULL. */
 void gemm_sm100_last_launch(int *grid, int *block, int *cluster);
 
 /* Selects the kernel family for this thread's later launches and returns the

@@ -17,6 +17,10 @@ constexpr int kBackwardBlocksPerSm = 2;
 constexpr int kMaxBackwardBlocks = 512;  // bounds the partial sums whatever the device
 constexpr int kLongRowParts = 64;       // row strides of the long-row parameter sums
 
+// A call's first launch, for gemm_sm100_last_launch (the second one adds up the
+// partial sums).
+thread_local int t_grid = 0, t_block = 0;
+
 template <typename Kernel, typename... Args>
 cudaError_t launch(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                    Args... args)
@@ -32,6 +36,10 @@ cudaError_t launch(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (t_grid == 0) {
+        t_grid = static_cast<int>(grid.x * grid.y);
+        t_block = static_cast<int>(block.x * block.y);
+    }
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -226,6 +234,7 @@ cudaError_t run(const PtgLayerNorm &a, bool back, cudaStream_t stream)
     PtgDevice dev;
     if (!ptg_device(&dev))
         return cudaErrorNoDevice;
+    t_grid = 0;
     cudaError_t err;
     switch (a.dtype) {
     case DTYPE_FLOAT32: err = dispatch<float>(a, dev, back, stream); break;
@@ -234,7 +243,8 @@ cudaError_t run(const PtgLayerNorm &a, bool back, cudaStream_t stream)
     default: err = cudaErrorInvalidValue; break;
     }
     if (err == cudaSuccess)
-        ptg_record_launch(back ? "layer-norm-backward" : "layer-norm", false, a.dtype, 0, 0, 0);
+        ptg_record_launch(back ? "layer-norm-backward" : "layer-norm", false, a.dtype, t_grid,
+                          t_block, 1);
     return err;
 }
 

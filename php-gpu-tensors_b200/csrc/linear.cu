@@ -121,6 +121,7 @@ struct Plan {
     cudaError_t err;
     int parts, passes;      // float32: bfloat16 parts and products of them; else 1, 1
     const char *kernel;     // of the last product, for gemm_sm100_last_kernel
+    int grid, block, cluster;   // its launch, or the bias gradient's where there is none
     int dtype;
     LayParams lay[2];       // layouts that the next product waits for
     int lays;
@@ -130,6 +131,12 @@ struct Plan {
     {
         if (ok())
             err = e;
+    }
+    void note(unsigned blocks, int threads, int ctas)
+    {
+        grid = static_cast<int>(blocks);
+        block = threads;
+        cluster = ctas;
     }
 };
 
@@ -308,7 +315,7 @@ int pair_count(int sms)
 }
 
 template <typename T, bool INNER, bool CHUNKED>
-cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p, long long bound)
+cudaError_t launch_pairs(Plan &pl, const RaggedMaps &maps, RaggedParams &p, long long bound)
 {
     constexpr auto kernel = ragged_gemm_kernel<T, INNER, CHUNKED>;
     const int pairs = pair_count<kernel>(pl.dev.sms);
@@ -333,6 +340,7 @@ cudaError_t launch_pairs(const Plan &pl, const RaggedMaps &maps, RaggedParams &p
     cfg.stream = pl.stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
+    pl.note(cfg.gridDim.x, kRaggedThreads, 2);
     return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
 
@@ -347,7 +355,7 @@ uint32_t instruction(int dtype, bool a_mn, bool b_mn, int m)
 // The few-row kernel: how many CTAs share the inner axis of a tile.  As many
 // as keep two CTAs on every SM, and at least four k-blocks for each.
 template <typename T>
-cudaError_t launch_decode(const Plan &pl, const RaggedMaps &maps, RaggedParams &p)
+cudaError_t launch_decode(Plan &pl, const RaggedMaps &maps, RaggedParams &p)
 {
     constexpr auto kernel = ragged_decode_kernel<T>;
     static std::mutex mutex;
@@ -388,6 +396,7 @@ cudaError_t launch_decode(const Plan &pl, const RaggedMaps &maps, RaggedParams &
     cfg.stream = pl.stream;
     cfg.attrs = attr;
     cfg.numAttrs = split > 1 ? 2 : 1;
+    pl.note(cfg.gridDim.x, kDecodeThreads, split);
     return cudaLaunchKernelEx(&cfg, kernel, maps, p, split);
 }
 
@@ -406,7 +415,7 @@ bool few_rows(const PtgDevice &dev, long long pair_tiles, int rows, int groups)
 constexpr int kSimtFewRows = 16;
 
 template <typename T, typename TZ, bool INNER, int TF, int TR>
-cudaError_t launch_simt_tile(const Plan &pl, RaggedSimtParams &s)
+cudaError_t launch_simt_tile(Plan &pl, RaggedSimtParams &s)
 {
     constexpr auto kernel = ragged_simt_kernel<T, TZ, INNER, TF, TR>;
     static std::mutex mutex;
@@ -451,11 +460,12 @@ cudaError_t launch_simt_tile(const Plan &pl, RaggedSimtParams &s)
     cfg.stream = pl.stream;
     cfg.attrs = attr;
     cfg.numAttrs = s.split > 1 ? 2 : 1;
+    pl.note(cfg.gridDim.x, kSimtThreads, s.split);
     return cudaLaunchKernelEx(&cfg, kernel, s);
 }
 
 template <typename T, typename TZ, bool INNER>
-cudaError_t launch_simt_rows(const Plan &pl, RaggedSimtParams &s)
+cudaError_t launch_simt_rows(Plan &pl, RaggedSimtParams &s)
 {
     const int rows = INNER ? s.p.cols : (s.p.rows + s.p.groups - 1) / s.p.groups;
     return rows <= kSimtFewRows ? launch_simt_tile<T, TZ, INNER, 128, 16>(pl, s)
@@ -463,7 +473,7 @@ cudaError_t launch_simt_rows(const Plan &pl, RaggedSimtParams &s)
 }
 
 template <bool INNER>
-cudaError_t launch_simt(const Plan &pl, RaggedSimtParams &s, int dtype, bool z_f32)
+cudaError_t launch_simt(Plan &pl, RaggedSimtParams &s, int dtype, bool z_f32)
 {
     switch (dtype) {
     case DTYPE_FLOAT16:
@@ -844,6 +854,7 @@ void slope(Plan &pl, const PtgLinear &a, void *dz, int parts, float *partial)
     const dim3 grid(static_cast<unsigned>(p.strips) *
                     (a.rows / kSlopeRows + std::min(a.groups, a.rows)));
     const size_t table = static_cast<size_t>(a.groups) * 8;
+    pl.note(grid.x, 256, 1);
     switch (a.dtype) {
     case DTYPE_FLOAT16: pl.then(launch(slope_kernel<__half>, grid, 256, table, pl.stream, p)); break;
     case DTYPE_BFLOAT16:
@@ -944,7 +955,7 @@ cudaError_t sized_then_run(const PtgLinear &a, size_t *need, cudaStream_t stream
     body(pl, a);
     if (pl.ok())
         ptg_record_launch(pl.kernel ? pl.kernel : "linear-bias-gradient", pl.kernel != nullptr,
-                          a.dtype, 0, 0, 0);
+                          a.dtype, pl.grid, pl.block, pl.cluster);
     return pl.err;
 }
 

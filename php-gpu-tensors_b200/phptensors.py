@@ -774,8 +774,8 @@ def set_kernel_path(path):
 
 
 def last_launch():
-    """(grid, block, cluster) of the last tensor-core or few-column launch on
-    this thread."""
+    """(grid, block, cluster) of the last tensor-core, few-column or feed-forward
+    launch on this thread."""
     g, b, c = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
     library().gemm_sm100_last_launch(ctypes.byref(g), ctypes.byref(b), ctypes.byref(c))
     return g.value, b.value, c.value

@@ -582,3 +582,24 @@ def test_sizes_that_pass_32_bits_are_refused():
         assert lib.pt_linear_backward(ref(y), ref(x), ref(w), None, None, 0, ref(x), ref(w), None,
                                       None, ref(size), None) == P.PT_INVALID_ARGUMENT
         assert b"2^31" in lib.pt_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("path,block,clusters", [
+    ("tensor-core", 192, (1, 2, 4, 8)), ("tensor-core-pair", 608, (2,)),
+    ("simt", 256, (1, 2, 4, 8))], indirect=["path"])
+def test_last_launch(path, block, clusters):
+    """gemm_sm100_last_launch describes the product's launch, the bias
+    gradient's or the norm's where the call has no product."""
+    c = case(130, 512, 264, "bfloat16", 3)
+    for call in (lambda: arr(c["x"]).linear(arr(c["w"])),
+                 lambda: P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), weights=False)):
+        call()
+        grid, threads, cluster = P.last_launch()
+        assert threads == block and cluster in clusters and grid > 0 and grid % cluster == 0
+    P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), inputs=False, weights=False)
+    grid, threads, cluster = P.last_launch()
+    assert grid == 2 * 3 and threads == 256 and cluster == 1     # column strips x row tiles
+    arr(c["x"]).layer_norm()
+    grid, threads, cluster = P.last_launch()
+    assert 0 < grid <= 130 and threads in (256, 512) and cluster == 1
