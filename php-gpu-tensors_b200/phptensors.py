@@ -389,8 +389,11 @@ class CudaArray:
         if n > MAX_DIMS:
             raise InvalidArgumentException("tensors have at most %d axes" % MAX_DIMS)
         pad = _PAD[n]
-        return _PT_TENSOR.pack(self._address(), DTYPE_CODES[self._dtype], n, *self._shape, *pad,
-                               *self._strides, *pad)
+        try:
+            return _PT_TENSOR.pack(self._address(), DTYPE_CODES[self._dtype], n, *self._shape,
+                                   *pad, *self._strides, *pad)
+        except struct.error:
+            raise InvalidArgumentException("extents must be 32-bit and strides not negative")
 
     # ---------------------------------------------------------- matmul
     def matmul(self, other, allow_float64=False):
@@ -453,7 +456,7 @@ class CudaArray:
         """Layer norm over the last axis (pt_layer_norm); gamma and beta are
         [cols] arrays of this dtype or float32.  With save_stats the result is
         (y, mean, rstd), the float32 statistics layer_norm_backward takes."""
-        _check_feed_forward("layer_norm", self, gamma, beta)
+        _check_feed_forward("layer_norm", (), gamma, beta)
         y = _result_like(self)
         mean, rstd = _result_pair(self._shape[:-1]) if save_stats else (None, None)
         _raise_for(library().pt_layer_norm(
@@ -466,15 +469,14 @@ class CudaArray:
         self [..., K], weight [K, N], bias [N], residual [..., N]; activation
         one of ACTIVATIONS.  With save_pre the result is (y, pre), pre the
         pre-activation that linear_backward takes."""
-        return _linear(self, weight, None, bias, activation, residual, save_pre)
+        return _linear(self, weight, (), bias, activation, residual, save_pre)
 
     def grouped_linear(self, weight, ends, bias=None, activation="none", residual=None,
                        save_pre=False):
         """linear with an own weight [E, K, N] and bias [E, N] for each of E
         groups of consecutive rows of self [rows, K]; ends, an int32 torch
         tensor on the device, holds the row behind each group's last one."""
-        return _linear(self, weight, _check_ends(ends, weight), bias, activation, residual,
-                       save_pre)
+        return _linear(self, weight, (ends,), bias, activation, residual, save_pre)
 
     # ---------------------------------------------------------- export
     def to_torch(self):
@@ -499,10 +501,13 @@ class CudaArray:
 
 
 # ---------------------------------------------------------------- feed-forward
-def _check_feed_forward(what, *arrays):
-    for a in arrays:
-        if a is not None and not isinstance(a, CudaArray):
+def _check_feed_forward(what, required, *optional):
+    for a in required:
+        if not isinstance(a, CudaArray):
             raise InvalidArgumentException("%s operands must be CudaArrays" % what)
+    for a in optional:
+        if a is not None and not isinstance(a, CudaArray):
+            raise InvalidArgumentException("%s operands must be CudaArrays or None" % what)
 
 
 def _result(shape, dtype, like=None):
@@ -568,7 +573,7 @@ def layer_norm_backward(grad, x, gamma, mean, rstd, params=True):
     """Gradients of CudaArray.layer_norm (pt_layer_norm_backward): (dx, dgamma,
     dbeta), the last two float32 sums over all rows (None without `params`).
     mean and rstd are the statistics layer_norm saved."""
-    _check_feed_forward("layer_norm_backward", grad, x, gamma, mean, rstd)
+    _check_feed_forward("layer_norm_backward", (grad, x, mean, rstd), gamma)
     lead, cols = x._shape[:-1], x._shape[-1] if x._shape else 0
     for s in (mean, rstd):
         if s._dtype != "float32" or s._shape != lead or s._strides != _contiguous_strides(lead):
@@ -601,7 +606,7 @@ def _check_ends(ends, weight):
             or ends.dim() != 1 or not ends.is_contiguous()):
         raise InvalidArgumentException(
             "ends must be a contiguous int32 vector on the device, one value a group")
-    if isinstance(weight, CudaArray) and weight._shape[:1] != [ends.numel()]:
+    if weight._shape[:1] != [ends.numel()]:
         raise InvalidArgumentException("ends must have one value for each of the weight's groups")
     return ends.data_ptr()
 
@@ -619,7 +624,9 @@ def _with_workspace(call, args, stream):
 
 
 def _linear(x, weight, ends, bias, activation, residual, save_pre):
-    _check_feed_forward("linear", x, weight, bias, residual)
+    """ends: empty, or the one `ends` of a grouped layer."""
+    _check_feed_forward("linear", (weight,), bias, residual)
+    ends = _check_ends(*ends, weight) if ends else None
     if not x._shape or not weight._shape:
         raise InvalidArgumentException("linear layers require rows and a weight")
     code = _activation_code(activation)
@@ -634,8 +641,11 @@ def _linear(x, weight, ends, bias, activation, residual, save_pre):
 
 def _linear_backward(grad, x, weight, ends, pre, activation, bias, inputs, weights,
                      weight_grad_dtype):
-    _check_feed_forward("linear_backward", grad, x, weight, pre)
+    _check_feed_forward("linear_backward", (grad, x, weight), pre)
     code = _activation_code(activation)
+    if weight_grad_dtype is not None:
+        _check_dtype(weight_grad_dtype)
+    ends = _check_ends(*ends, weight) if ends else None
     dx = _result_like(x) if inputs else None
     dw = None
     if weights:
@@ -654,14 +664,14 @@ def linear_backward(grad, x, weight, pre=None, activation="none", bias=True, inp
     None where it is not wanted (inputs, weights, bias).  pre is what
     linear(save_pre=True) kept; dw has weight's type or float32, dbias is
     float32; the residual's gradient is grad itself."""
-    return _linear_backward(grad, x, weight, None, pre, activation, bias, inputs, weights,
+    return _linear_backward(grad, x, weight, (), pre, activation, bias, inputs, weights,
                             weight_grad_dtype)
 
 
 def grouped_linear_backward(grad, x, weight, ends, pre=None, activation="none", bias=True,
                             inputs=True, weights=True, weight_grad_dtype=None):
     """Gradients of CudaArray.grouped_linear, as linear_backward."""
-    return _linear_backward(grad, x, weight, _check_ends(ends, weight), pre, activation, bias,
+    return _linear_backward(grad, x, weight, (ends,), pre, activation, bias,
                             inputs, weights, weight_grad_dtype)
 
 

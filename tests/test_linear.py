@@ -603,3 +603,26 @@ def test_last_launch(path, block, clusters):
     arr(c["x"]).layer_norm()
     grid, threads, cluster = P.last_launch()
     assert 0 < grid <= 130 and threads in (256, 512) and cluster == 1
+
+
+def test_python_refusals():
+    """What is missing or of another kind is refused as an argument, before
+    torch or the device are asked for anything."""
+    def host(*shape, dtype="float32"):
+        return P.CudaArray(torch.zeros(math.prod(shape)), shape, dtype=dtype)
+    x, w, y = host(4, 8), host(8, 16), host(4, 16)
+    stats = host(4)
+    for call in (lambda: x.linear(None), lambda: x.grouped_linear(None, None),
+                 lambda: x.linear(w, bias=torch.zeros(16)),
+                 lambda: P.linear_backward(None, x, w), lambda: P.linear_backward(y, None, w),
+                 lambda: P.linear_backward(y, x, None),
+                 lambda: P.linear_backward(y, x, w, weight_grad_dtype="int8"),
+                 lambda: P.grouped_linear_backward(y, x, None, None),
+                 lambda: P.grouped_linear_backward(None, x, w, None),
+                 lambda: P.layer_norm_backward(None, x, None, stats, stats),
+                 lambda: P.layer_norm_backward(x, None, None, stats, stats),
+                 lambda: P.layer_norm_backward(x, x, None, None, stats),
+                 lambda: P.layer_norm_backward(x, x, None, stats, None),
+                 lambda: x.view([2, 8], [-8, 1], 8)._packed()):
+        with pytest.raises(P.InvalidArgumentException):
+            call()
