@@ -277,3 +277,25 @@ def test_sizes_that_pass_32_bits_are_refused():
     assert lib.pt_layer_norm_backward(ref(x), ref(x), None, 16, 16, ref(x), 16, 16, None,
                                       ref(size), None) == P.PT_INVALID_ARGUMENT
     assert b"2^31" in lib.pt_last_error()
+
+
+@gpu
+def test_parameter_gradients_beyond_32_bits():
+    """Sums over 2.2e9 elements as wholes: rows left out behind element 2^31, 3 %
+    of them, would be 17 % of dbeta's norm and 3 % of dgamma's.  A sum is joined
+    from chains of fewer than 1000 additions in float32, each within e of a
+    partial sum that is no larger than the whole in the mean: below 1000 e."""
+    rows, cols = 270001, 8192
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(rows, cols, generator=g, device="cuda", dtype=torch.bfloat16)
+    y, mean, rstd = arr(x).layer_norm(save_stats=True)
+    dx, dg, db = P.layer_norm_backward(y, arr(x), None, mean, rstd)
+    grad, m, r = y.to_torch(), mean.to_torch(), rstd.to_torch()
+    sums = torch.zeros(2, cols, device="cuda").double()
+    for at in range(0, rows, 15000):
+        part = slice(at, at + 15000)
+        dy = grad[part].double()
+        sums[0] += (dy * ((x[part].double() - m[part, None]) * r[part, None].double())).sum(0)
+        sums[1] += dy.sum(0)
+    for got, want in ((dg, sums[0]), (db, sums[1])):
+        assert (got.to_torch().double() - want).norm() <= 1000 * E * want.norm()
