@@ -626,3 +626,55 @@ def test_python_refusals():
                  lambda: x.view([2, 8], [-8, 1], 8)._packed()):
         with pytest.raises(P.InvalidArgumentException):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("path", ["auto", "tensor-core", "tensor-core-pair"], indirect=True)
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("rows,inner,cols,ends", [
+    (300, 128, 320, [0, 70, 70, 71, 260]),          # chunked maps, three feature tiles of dx
+    (3200, 256, 192, [1500, 1501, 3190]),           # a group's rows in parts for dw
+    (40, 1024, 384, [3, 3, 20, 37])])               # few rows, the inner axis over a cluster
+def test_grouped_widths_of_64(dtype, path, rows, inner, cols, ends):
+    """Widths that are multiples of 64, as real experts have them: operands
+    whose maps walk chunks of 64 beside the group's coordinate, as they lie
+    and with the weight transposed."""
+    at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    spans = spans_of(ends, rows)
+    for layout in ("plain", "column"):
+        c = case(rows, inner, cols, dtype, 41, groups=len(ends))
+        c["w"] = strided(c["w"], layout)
+        for k in ("x", "grad", "pre", "res"):
+            c[k][spans[-1][1]:] = float("nan")
+        y, pre = arr(c["x"]).grouped_linear(arr(c["w"]), at, arr(c["bias"]), "silu",
+                                            arr(c["res"]), save_pre=True)
+        check_forward(c, y.to_torch(), pre.to_torch(), dtype, "silu", spans)
+        for act in ("silu", "none"):
+            out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at,
+                                            arr(c["pre"]), act)
+            check_backward(c, out, dtype, act, spans)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("groups", [None, 3])
+def test_more_tiles_than_pairs(dtype, groups):
+    """Every pair takes several tiles of eight k-blocks and more, both
+    accumulators in turn."""
+    rows, inner, cols = 2100, 576, 4352
+    ends = [rows] if groups is None else [700, 1405, 2099]
+    spans = spans_of(ends, rows)
+    c = case(rows, inner, cols, dtype, 43, groups=groups)
+    before = P.set_kernel_path("tensor-core-pair")
+    try:
+        if groups is None:
+            y = arr(c["x"]).linear(arr(c["w"]), arr(c["bias"]), "none", arr(c["res"]))
+            out = P.linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]))
+        else:
+            at = torch.tensor(ends, dtype=torch.int32, device="cuda")
+            y = arr(c["x"]).grouped_linear(arr(c["w"]), at, arr(c["bias"]), "none", arr(c["res"]))
+            out = P.grouped_linear_backward(arr(c["grad"]), arr(c["x"]), arr(c["w"]), at)
+    finally:
+        P.library().gemm_sm100_set_path(before)
+    check_forward(c, y.to_torch(), None, dtype, "none", spans)
+    check_backward(c, out, dtype, "none", spans)
