@@ -678,3 +678,17 @@ def test_more_tiles_than_pairs(dtype, groups):
         P.library().gemm_sm100_set_path(before)
     check_forward(c, y.to_torch(), None, dtype, "none", spans)
     check_backward(c, out, dtype, "none", spans)
+
+
+@gpu
+@pytest.mark.parametrize("act", sorted(set(P.ACTIVATIONS) - {"none", "relu"}))
+@pytest.mark.parametrize("dtype", ALL)
+def test_slopes_are_float32(dtype, act):
+    """dbias sums slopes in float32, so these are held to float32 whatever the
+    operands' type: a few roundings and an exponential within (|x| + 4) 2^-23 come
+    to some 2^-23 of their norm; a fit made for 16-bit results would be
+    ten times that."""
+    g = torch.Generator(device="cuda").manual_seed(51)
+    z = torch.randn(1 << 16, generator=g, device="cuda").to(DT[dtype])
+    want = slope64(z.double(), act)
+    assert (slope_of(act, z, dtype) - want).norm() <= 2.0 ** -22.5 * want.norm()
