@@ -63,10 +63,13 @@ size_t pt_layer_norm_backward_workspace(long long rows, int cols);
  * workspace first, and so are the bfloat16 parts of float32 ones.
  *
  * bias is contiguous [N] ([E, N]) of x's type or float32; residual has y's
- * shape and x's type; activation is a CUDA_MATMUL_EPILOGUE_* value.  y and,
- * unless NULL, pre = x . w + bias, which the backward pass needs for an
- * activation, are [..., N] of x's type.  Infinite float32 operands can turn
- * to NaN as in the strict mode of cuda_blas_set_precision.
+ * shape and x's type; activation is a CUDA_MATMUL_EPILOGUE_* value.  RELU is
+ * z > 0 ? z : 0 as in the matmul's epilogue, so that NaN becomes 0 there (and its
+ * slope 0); the other activations keep it.  y and, unless NULL,
+ * pre = x . w + bias, which the backward pass needs for an activation, are
+ * [..., N] of x's type.  Infinite float32 operands, and finite ones that round to
+ * infinity in bfloat16 (from 3.396e38 on), can turn to NaN as in the strict mode of
+ * cuda_blas_set_precision.
  *
  * *workspace_bytes holds the size of `workspace` (16-byte aligned); where it
  * is too small the call returns PT_WORKSPACE with the need in its place. */

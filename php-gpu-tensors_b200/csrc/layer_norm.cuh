@@ -18,11 +18,14 @@
 // launch adds the partial rows in order (no atomics: the result does not
 // depend on timing).
 //
-// On B200: 16384 x 4096 bfloat16 backwards 84 us and 5 us for the partial rows (403 MB
-// are 62 us at the copy rate; what is left is loads in flight: one row ahead
-// is what 128 registers hold, and rows brought ahead into shared memory
-// by bulk copies ran slower, 116 us, before the arithmetic was packed); 3001 x 1531
-// float32 forwards 16.5 us (5.6), of which a launch takes about five.
+// On B200, with the time of the bytes at the copy rate behind it: 16384 x 4096
+// bfloat16 forwards 84 us (41), backwards 84 and 5 for the partial rows (62); one
+// row ahead is what the registers hold, and more loads in flight have been tried
+// only before the arithmetic was packed (bulk copies into shared memory, 116 us).
+// 3001 x 1531 float32 forwards 14 us (5.6) and 17 alone, of which a launch takes
+// about five: 4-byte loads, as its rows start at every alignment.  8192 x 1024
+// float32 16 (10) and 26 (15); 4096 x 12288 bfloat16 61 (31) and, on the kernels for
+// long rows with their three reads of single elements, 340 (46).
 #pragma once
 
 #include "ptx_sm100.cuh"

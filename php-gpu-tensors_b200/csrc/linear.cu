@@ -402,9 +402,9 @@ cudaError_t launch_decode(Plan &pl, const RaggedMaps &maps, RaggedParams &p)
 
 // Few rows: at most a quarter of a tile's on average, or two tiles' when the
 // pair kernel would not occupy the GPU once.  Measured on B200 (us, few rows /
-// pairs): one 4096 x 4096 weight, 16 rows 9.2 / 20.5, 64 rows 12.7 / 21.9, 128
-// rows 17.6 / 21.9, 256 rows 27.6 / 23.0; 32 experts of 2048 x 1024, 32 rows
-// 16.8 / 24.1, 1024 rows 35.6 / 30.5.
+// pairs, weights from memory): one 4096 x 4096 weight, 16 rows 11 / 22, 64 rows 14 /
+// 23, 128 rows 18 / 23, 256 rows 27 / 24; 32 experts of 2048 x 1024, 32 rows 20 / 28,
+// 1024 rows 36 / 31.
 bool few_rows(const PtgDevice &dev, long long pair_tiles, int rows, int groups)
 {
     return rows <= kDecodeRows / 4 * static_cast<long long>(groups) ||
@@ -758,10 +758,15 @@ bool begin(Plan &pl, const PtgLinear &a, bool run, cudaStream_t stream)
 
 // Whether a product runs on the CUDA cores: float32 ones below kSimtWork
 // multiply-adds, 16-bit ones below kSimtLayWork whose operands would have to
-// be laid out first.  Measured on B200 (us, CUDA cores / three parts on the tensor
-// cores): 8 x 4096 x 4096 37 / 171, 64 x 1024 x 1024 20 / 37, 512 x 1024 x 1024
-// 50 / 49, 1024 x 1024 x 1024 90 / 52.  The thread's kernel path decides first (2:
-// CUDA cores, 1 and 3: the tensor-core kernels).
+// be laid out first.  The bound lies where the two cross for weights of a million
+// elements; measured on B200 (us, CUDA cores / three parts on the tensor cores): 64 x
+// 1024 x 1024 15 / 37, 512 x 1024 x 1024 49 / 41, 1024 x 1024 x 1024 90 / 43; 16 experts of
+// 1024 x 1024, 256 rows 64 / 88, 2048 rows 213 / 108.  For larger weights, whose parts
+// the tensor cores' path writes and reads again on every call, they cross at more work
+// than the bound, and between the two it takes the slower side: 8 x 4096 x 4096 38 /
+// 139 (CUDA cores), but 64 x 4096 x 4096 89 / 144, 8 x 8192 x 8192 142 / 341 and 64 experts
+// of 2048 x 1408 with 2048 rows 782 / 834 (tensor cores).  The thread's kernel path
+// decides first (2: CUDA cores, 1 and 3: the tensor-core kernels).
 constexpr double kSimtWork = 5.0e8;
 constexpr double kSimtLayWork = 5.0e7;
 

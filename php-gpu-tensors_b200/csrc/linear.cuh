@@ -173,9 +173,10 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, int 
 // gradient, the column sums of dz before that rounding, in float32.  A block
 // takes 64 rows of one group and 256 columns, 8 a thread in 8 row lanes, and
 // writes one partial row; group_sums_kernel adds a group's partial rows in
-// order.  grad and z are read and dz written once each: 8192 x 8192 bfloat16 with
-// gelu_tanh takes 94 us on B200, 62 at the copy rate; the derivative's
-// instructions (some 25 an element) take about as long as the loads.
+// order.  grad and z are read and dz written once each: 8192 x 8192 bfloat16 takes
+// 83 us with gelu_tanh on B200, 103 with gelu, 66-73 with the others, 62 at the copy
+// rate; the derivative's instructions (25 to 35 an element) take about as long as
+// the loads.
 constexpr int kSlopeRows = 64;
 constexpr int kSlopeCols = 256;
 

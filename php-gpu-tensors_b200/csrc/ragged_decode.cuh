@@ -10,8 +10,9 @@
 // CTAs in rank order (the result does not depend on timing) and finishing
 // them.  96 KB of tiles in flight per CTA and two CTAs per SM keep
 // enough loads outstanding for the memory's latency: 8 x 4096 x 4096 bfloat16 takes
-// 8.5-10.5 us with its launch (the weight's 34 MB alone 5.1 at the copy rate),
-// where the pair kernel's 16 tiles take 20.
+// 10.4 us in a run of calls on weights that come from memory (8.5 where L2 has
+// them; alone, with its launch, 14), the weight's 34 MB 5.1 at the copy rate; the
+// pair kernel's 16 tiles take 21.
 #pragma once
 
 #include "ragged_gemm.cuh"

@@ -18,11 +18,12 @@
 // residual and store.  Barriers as in gemm_tc2.cuh; every wait is bounded.  No
 // TMA multicast.
 //
-// On B200: 8192^3 bfloat16 709-737 us = 1.49-1.55 PFLOP/s, where the power cap sets
-// the clock; 16384 x 2048 x 8192 with gelu and the pre-activation stored 425-440
-// us; 64 experts, 8192 rows, 2048 x 1408 88-95 us for 370 MB of weights, where
-// what a k-block costs the threads that issue loads and MMAs, and a last round
-// of tiles that is mostly empty, keep it from the memory's rate.
+// On B200, GPU time of short runs (the power cap makes a long one of large products
+// 10-20 % slower): 8192^3 bfloat16 707-737 us = 1.49-1.56 PFLOP/s; 16384 x 2048 x 8192
+// with gelu_tanh and the pre-activation stored 424 us (492-522 in a long run), with
+// gelu 431-483; 64 experts, 8192 rows, 2048 x 1408 84-95 us for 370 MB of weights,
+// where what a k-block costs the threads that issue loads and MMAs, and a last
+// round of tiles that is mostly empty, keep it from the memory's rate.
 //
 // Ragged INNER axis: a k-block that crosses the end of its group must not
 // meet the next group's rows (they may hold NaN, so a zero on one side is
@@ -36,7 +37,8 @@
 // 2^-16.  The tensor core truncates its accumulator at every instruction, so
 // it is restarted every kChunkBlocks k-blocks and the epilogue adds the chunks
 // in registers, rounding to nearest: 2.7e-7 of the result's norm from float64 at
-// K = 1024.  8192 x 4096 x 4096: 1160 us = 237 TFLOP/s, 1.42 PFLOP/s of MMAs.
+// K = 1024.  8192 x 4096 x 4096: 1130-1160 us = 237-243 TFLOP/s, 1.42-1.46 PFLOP/s of
+// MMAs.
 #pragma once
 
 #include "activation.cuh"
